@@ -17,6 +17,8 @@ MATH_EXPF, MATH_SQRT, MATH_DIV, MATH_SILU, MATH_F16 = 0, 1, 2, 3, 4
 ROUTE_AUTO, ROUTE_EXACT, ROUTE_FORCE_FALLBACK, ROUTE_FORCE_REFINE = 0, 1, 2, 3
 EXPERTS_AUTO, EXPERTS_GEMV, EXPERTS_MFMA = 0, 1, 2
 ATTN_PER_HEAD, ATTN_SPLIT = 0, 1
+T_F32, T_F16, T_BF16 = 0, 1, 2
+ROPE_HALVES, ROPE_ADJACENT = 0, 1
 KT_ROUTE, KT_SELECT, KT_GATEUP, KT_DOWN, KT_COMBINE, KT_FUSED, KT_COUNT = 0, 1, 2, 3, 4, 5, 6
 KT_NAMES = ("route", "select", "gateup", "down", "combine", "fused")
 BLOCK_BYTES = {ENC_Q4: 18, ENC_Q8: 34}
@@ -36,6 +38,7 @@ class CPGError(RuntimeError):
 
 _c = ctypes
 _vp, _i, _sz, _u64, _f, _d = _c.c_void_p, _c.c_int, _c.c_size_t, _c.c_uint64, _c.c_float, _c.c_double
+_i64 = _c.c_int64
 
 # (name, restype, argtypes) for every entry point of include/cpg.h
 SIGNATURES = [
@@ -101,6 +104,11 @@ SIGNATURES = [
     ("cpg_capture_end", _vp, []),
     ("cpg_graph_launch", _i, [_vp]),
     ("cpg_graph_destroy", None, [_vp]),
+    ("cpg_paged_ws_create", _vp, [_i, _i, _i]),
+    ("cpg_paged_ws_destroy", None, [_vp]),
+    ("cpg_paged_ws_status", _i, [_vp]),
+    ("cpg_paged_append", _i, [_vp, _vp, _vp, _i, _i, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp]),
+    ("cpg_paged_attn", _i, [_vp, _vp, _i, _i, _vp, _i64, _f, _i, _vp, _i64, _vp, _vp]),
 ]
 
 
@@ -115,6 +123,25 @@ class MoELayer(ctypes.Structure):
     """cpg_moe_layer of include/cpg.h"""
     _fields_ = [("D", _i), ("E", _i), ("K", _i), ("F", _i), ("enc", _i), ("eps", _f),
                 ("ln2", _vp), ("wgate", _vp), ("experts", _vp)]
+
+
+class PagedCache(ctypes.Structure):
+    """cpg_paged_cache of include/cpg.h"""
+    _fields_ = [("KV", _i), ("HD", _i), ("type", _i), ("page", _i), ("n_pages", _i),
+                ("page_stride", _i64), ("slot_stride", _i64), ("head_stride", _i64), ("k", _vp),
+                ("v", _vp)]
+
+
+class PagedBatch(ctypes.Structure):
+    """cpg_paged_batch of include/cpg.h"""
+    _fields_ = [("S", _i), ("T", _i), ("max_new", _i), ("max_pages", _i), ("pages", _vp),
+                ("q_off", _vp), ("len", _vp)]
+
+
+class PagedRope(ctypes.Structure):
+    """cpg_paged_rope of include/cpg.h"""
+    _fields_ = [("table", _vp), ("max_pos", _i), ("rot", _i), ("pairs", _i), ("q_norm", _vp),
+                ("k_norm", _vp), ("eps", _f)]
 
 
 _lib = None

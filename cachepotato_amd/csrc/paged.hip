@@ -1,0 +1,366 @@
+/* paged.hip — the paged key/value cache: the new tokens' heads into it (cpg_paged_append), and the
+ * host side of the attention over it (cpg_paged_attn, whose kernels are in paged_few.hip).
+ */
+#include "cpg_paged.h"
+
+#include <math.h>
+#include <stdlib.h>
+
+/* ---------------------------------------------------------------- append */
+
+struct pg_append {
+    const void *q, *k, *v;
+    void *q_out, *kc, *vc;
+    const int *pages, *q_off, *len;
+    int64_t ldq, ldk, ldv, ldqo, page_stride, slot_stride, head_stride;
+    const float *table, *q_norm, *k_norm;
+    int H, KV, HD, S, T, max_pages, n_pages, plog, max_pos, rot, adjacent, *stat;
+    float eps;
+};
+
+/* The last sequence s with q_off[s] <= t (-1: none), for ascending q_off: 64 probes a step, so one
+   step up to 64 sequences and two up to 4096. Whole wavefront. */
+__device__ static inline int pg_row_seq(const int *__restrict__ q_off, int S, int t) {
+    const int lane = threadIdx.x & 63;
+    int lo = 0, n = S;                           /* the answer is lo - 1 or in [lo, lo + n) */
+    while (n > 0) {
+        const int step = (n + 63) >> 6, i = lo + lane * step;
+        const bool yes = i < lo + n && q_off[i] <= t;
+        const int c = __popcll(__ballot(yes));
+        if (c == 0) return lo - 1;
+        const int end = lo + n;
+        lo += (c - 1) * step + 1;                /* probe c - 1 said yes, probe c no */
+        n = min(step - 1, end - lo);
+    }
+    return lo - 1;
+}
+
+/* grid (T, parts of the H + 2 KV heads), 256 threads: row t, 2^gl lanes to a head, eight elements a
+   lane (HD = 96 and 192 leave a quarter of the lanes idle). A query or key head is normed (its sum
+   of squares over the lanes in fp32), turned, and rounded once where it is stored; a value head is
+   only stored. The partner of a lane's elements in the rotation is a lane's whole eight, since rot
+   is a multiple of 16: rot / 16 lanes away, or its own.
+   Bound by the bytes of the heads in and out; for a few rows by the chain of launch, row's
+   sequence, page id, store. */
+template <int AT, int CT>
+__global__ __launch_bounds__(256) void k_paged_append(const pg_append a, int gl) {
+    const int t = blockIdx.x, tid = threadIdx.x, li = tid & ((1 << gl) - 1);
+    const int head = (blockIdx.y * 256 + tid) >> gl, heads = a.H + 2 * a.KV;
+    const bool live = head < heads && li * 8 < a.HD;
+    const int hc = min(head, heads - 1), lc = min(li, a.HD / 8 - 1);
+    const bool isq = hc < a.H, isv = hc >= a.H + a.KV;
+    const int hh = isq ? hc : isv ? hc - a.H - a.KV : hc - a.H;
+    typedef typename pg_elem<AT>::t at;
+    const at *src = (const at *)(isq ? a.q : isv ? a.v : a.k) +
+                    (size_t)t * (isq ? a.ldq : isv ? a.ldv : a.ldk) + (size_t)hh * a.HD + 8 * lc;
+    const int s = pg_row_seq(a.q_off, a.S, t);
+    if (s < 0) return;
+    const pg_seq sq = pg_get_seq(a.q_off, a.len, s, a.T, a.max_pages, a.plog);
+    if (t < sq.lo || t >= sq.lo + sq.n) {        /* a row of no sequence */
+        if (sq.bad && tid == 0) *a.stat = 1;
+        return;
+    }
+    const int pos = sq.p0 + t - sq.lo;
+    const bool bad = sq.bad || pos < 0 || (a.rot > 0 && pos >= a.max_pos);
+    const int pc = bad ? 0 : pos;
+    const int page = bad ? -1 : a.pages[(size_t)s * a.max_pages + (pc >> a.plog)];
+    const bool miss = page < 0 || page >= a.n_pages;
+    if (miss && tid == 0) *a.stat = 1;
+    float x[8];
+    if constexpr (AT == CPG_T_F32) {
+        const float4 u = ((const float4 *)src)[0], w = ((const float4 *)src)[1];
+        x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
+        x[4] = w.x; x[5] = w.y; x[6] = w.z; x[7] = w.w;
+    } else {
+        const uint4 u = *(const uint4 *)src;
+        const uint32_t uw[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float2 f = pg_unpack2<AT>(uw[i]);
+            x[2 * i] = f.x;
+            x[2 * i + 1] = f.y;
+        }
+    }
+    const float *gain = isq ? a.q_norm : a.k_norm;
+    if (gain && !isv) {
+        float ss = 0.0f;
+        if (li * 8 < a.HD)
+#pragma unroll
+            for (int i = 0; i < 8; i++) ss = fmaf(x[i], x[i], ss);
+        for (int o = 1; o < 1 << gl; o <<= 1) ss += __shfl_xor(ss, o);
+        const float inv = __fdiv_rn(1.0f, cpg_sqrt_rn(__fadd_rn(__fdiv_rn(ss, (float)a.HD), a.eps)));
+        const float4 g0 = ((const float4 *)gain)[2 * lc], g1 = ((const float4 *)gain)[2 * lc + 1];
+        const float g[8] = {g0.x, g0.y, g0.z, g0.w, g1.x, g1.y, g1.z, g1.w};
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = __fmul_rn(__fmul_rn(x[i], inv), g[i]);
+    }
+    if (a.rot > 0) {                             /* shuffles: every lane takes part */
+        const bool turn = !isv && 8 * li < a.rot;
+        const float4 *row = (const float4 *)(a.table + (size_t)pc * a.rot);
+        if (a.adjacent) {
+            const int c = turn ? 2 * li : 0;     /* pairs 4 li .. 4 li + 3, two to a float4 */
+            const float4 r0 = row[c], r1 = row[c + 1];
+            const float cs[8] = {r0.x, r0.y, r0.z, r0.w, r1.x, r1.y, r1.z, r1.w};
+            if (turn)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float u = x[2 * i], w = x[2 * i + 1], cc = cs[2 * i], sn = cs[2 * i + 1];
+                    x[2 * i] = __fsub_rn(__fmul_rn(u, cc), __fmul_rn(w, sn));
+                    x[2 * i + 1] = __fadd_rn(__fmul_rn(w, cc), __fmul_rn(u, sn));
+                }
+        } else {
+            const int hl = a.rot / 16;           /* lanes of half the rotated elements */
+            const bool upper = li >= hl;
+            const int c = turn ? 4 * (upper ? li - hl : li) : 0;
+            const int lane = tid & 63, other = turn ? (upper ? lane - hl : lane + hl) : lane;
+            float cs[16];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float4 r = row[c + i];
+                cs[4 * i] = r.x; cs[4 * i + 1] = r.y; cs[4 * i + 2] = r.z; cs[4 * i + 3] = r.w;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float y = __shfl(x[i], other), cc = cs[2 * i], sn = cs[2 * i + 1];
+                const float down = __fsub_rn(__fmul_rn(x[i], cc), __fmul_rn(y, sn));
+                const float up = __fadd_rn(__fmul_rn(x[i], cc), __fmul_rn(y, sn));
+                x[i] = turn ? (upper ? up : down) : x[i];
+            }
+        }
+    }
+    if (!live) return;
+    if (isq) {
+        if (bad)
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = __int_as_float(0x7fc00000);
+        const size_t e = (size_t)t * a.ldqo + (size_t)hh * a.HD + 8 * li;
+        pg_put4<AT>(a.q_out, e, make_float4(x[0], x[1], x[2], x[3]));
+        pg_put4<AT>(a.q_out, e + 4, make_float4(x[4], x[5], x[6], x[7]));
+    } else if (!miss) {
+        const size_t e = (size_t)page * a.page_stride +
+                         (size_t)(pos & ((1 << a.plog) - 1)) * a.slot_stride +
+                         (size_t)hh * a.head_stride + 8 * li;
+        void *dst = isv ? a.vc : a.kc;
+        pg_put4<CT>(dst, e, make_float4(x[0], x[1], x[2], x[3]));
+        pg_put4<CT>(dst, e + 4, make_float4(x[4], x[5], x[6], x[7]));
+    }
+}
+
+/* ---------------------------------------------------------------- host side */
+
+static int elem_bytes(int type) { return type == CPG_T_F32 ? 4 : 2; }
+
+static bool types_ok(int type, int cache) {
+    return (type == CPG_T_F32 && cache >= CPG_T_F32 && cache <= CPG_T_BF16) ||
+           ((type == CPG_T_F16 || type == CPG_T_BF16) && cache == type);
+}
+
+static bool head_dim_ok(int HD) { return HD == 64 || HD == 96 || HD == 128 || HD == 192 || HD == 256; }
+
+static bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
+
+/* rows of `heads` heads, `ld` elements apart, at p */
+static bool rows_ok(const void *p, int64_t ld, int heads, int HD, int type) {
+    return p && aligned16(p) && ld >= (int64_t)heads * HD && ld * elem_bytes(type) % 16 == 0;
+}
+
+/* the checks that both entry points make, of the arguments and then of the workspace; 0, or -1
+   with the reason set */
+static int check_call(const char *who, const cpg_paged_cache *C, const cpg_paged_batch *B, int type) {
+    if (!C || !B || !C->k || !C->v) {
+        cpg_set_error("%s: null argument", who);
+        return -1;
+    }
+    if (!types_ok(type, C->type)) {
+        cpg_set_error("%s: activations of type %d with a cache of type %d", who, type, C->type);
+        return -1;
+    }
+    if (!head_dim_ok(C->HD) || C->KV <= 0) {
+        cpg_set_error("%s: KV=%d, HD=%d (64, 96, 128, 192 or 256)", who, C->KV, C->HD);
+        return -1;
+    }
+    if (C->page <= 0 || C->page > 1024 || (C->page & (C->page - 1)) || C->n_pages <= 0) {
+        cpg_set_error("%s: %d pages of %d tokens (a power of two up to 1024)", who, C->n_pages, C->page);
+        return -1;
+    }
+    const int eb = elem_bytes(C->type);
+    const int64_t st[3] = {C->page_stride, C->slot_stride, C->head_stride};
+    const int64_t n[3] = {C->n_pages, C->page, C->KV};
+    for (int i = 0; i < 3; i++) {
+        if (st[i] * eb % 16 || (n[i] > 1 && st[i] < C->HD) || st[i] < 0 ||
+            (n[i] > 1 && st[i] > ((int64_t)1 << 56) / n[i])) {
+            cpg_set_error("%s: stride %lld (at least HD elements, a multiple of 16 bytes)", who,
+                          (long long)st[i]);
+            return -1;
+        }
+    }
+    if (!aligned16(C->k) || !aligned16(C->v)) {
+        cpg_set_error("%s: the pool is not aligned to 16 bytes", who);
+        return -1;
+    }
+    if (B->S < 0 || B->T < 0 || B->T > PG_MAX_LEN || B->max_pages < 0 ||
+        (B->S > 0 && B->T > 0 && (!B->q_off || !B->len || !B->pages || B->max_pages == 0))) {
+        cpg_set_error("%s: bad batch S=%d T=%d max_pages=%d", who, B->S, B->T, B->max_pages);
+        return -1;
+    }
+    return 0;
+}
+
+static int check_ws(const char *who, const cpg_paged_ws *ws, int H, const cpg_paged_cache *C) {
+    if (!ws) {
+        cpg_set_error("%s: null workspace", who);
+        return -1;
+    }
+    if (H != ws->H || C->KV != ws->KV || C->HD != ws->HD) {
+        cpg_set_error("%s: H=%d KV=%d HD=%d, the workspace's H=%d KV=%d HD=%d", who, H, C->KV, C->HD,
+                      ws->H, ws->KV, ws->HD);
+        return -1;
+    }
+    return 0;
+}
+
+static int log2_of(int x) {
+    int l = 0;
+    while ((1 << l) < x) l++;
+    return l;
+}
+
+extern "C" cpg_paged_ws *cpg_paged_ws_create(int H, int KV, int HD) {
+    if (!g_cpg.ready) { cpg_set_error("cpg_init has not been called"); return nullptr; }
+    if (H <= 0 || KV <= 0 || H % KV || !head_dim_ok(HD) || H > 65536) {
+        cpg_set_error("cpg_paged_ws_create: bad geometry H=%d KV=%d HD=%d", H, KV, HD);
+        return nullptr;
+    }
+    cpg_paged_ws *ws = (cpg_paged_ws *)calloc(1, sizeof *ws);
+    if (!ws) { cpg_set_error("out of host memory"); return nullptr; }
+    ws->H = H;
+    ws->KV = KV;
+    ws->HD = HD;
+    ws->rows = (size_t)2 * PG_FEW_WGS * PG_FEW_ROWS;
+    const size_t sz[6] = {ws->rows * HD * 4, ws->rows * 8, PG_FEW_WGS * 4, 4, 1024, 1024};
+    size_t total = 0;
+    for (int i = 0; i < 6; i++) total += cpg_round256(sz[i]);
+    uint8_t *p = (uint8_t *)cpg_malloc(total);
+    if (!p) { free(ws); return nullptr; }
+    ws->block = p;
+    void **dst[6] = {(void **)&ws->pacc, (void **)&ws->pml, (void **)&ws->ctr, (void **)&ws->stat,
+                     (void **)&ws->zeros, (void **)&ws->nans};
+    for (int i = 0; i < 6; i++) {
+        *dst[i] = p;
+        p += cpg_round256(sz[i]);
+    }
+    /* nans: every bit set is a NaN in all three element types */
+    if (cpg_memset(ws->ctr, 0, sz[2]) || cpg_memset(ws->stat, 0, 4) ||
+        cpg_memset(ws->zeros, 0, 1024) || cpg_memset(ws->nans, 255, 1024)) {
+        cpg_paged_ws_destroy(ws);
+        return nullptr;
+    }
+    return ws;
+}
+
+extern "C" void cpg_paged_ws_destroy(cpg_paged_ws *ws) {
+    if (!ws) return;
+    cpg_free(ws->block);
+    free(ws);
+}
+
+extern "C" int cpg_paged_ws_status(cpg_paged_ws *ws) {
+    CPG_REQUIRE_INIT();
+    if (!ws) { cpg_set_error("cpg_paged_ws_status: null workspace"); return -1; }
+    int v = 0;
+    if (cpg_sync() || cpg_d2h(&v, ws->stat, sizeof v)) return -7;
+    if (v && cpg_memset(ws->stat, 0, sizeof v)) return -7;
+    return v;
+}
+
+extern "C" int cpg_paged_append(const cpg_paged_cache *C, const cpg_paged_batch *B,
+                                const cpg_paged_rope *R, int type, int H, const void *q, int64_t ldq,
+                                const void *k, int64_t ldk, const void *v, int64_t ldv, void *q_out,
+                                int64_t ldqo, cpg_paged_ws *ws) {
+    if (check_call("cpg_paged_append", C, B, type)) return -1;
+    if (H < 0 || H > 65536) { cpg_set_error("cpg_paged_append: %d query heads", H); return -1; }
+    if (!rows_ok(k, ldk, C->KV, C->HD, type) || !rows_ok(v, ldv, C->KV, C->HD, type) ||
+        (H && (!rows_ok(q, ldq, H, C->HD, type) || !rows_ok(q_out, ldqo, H, C->HD, type)))) {
+        cpg_set_error("cpg_paged_append: rows of heads must not be null or overlap, and start on 16 bytes");
+        return -1;
+    }
+    pg_append a = {};
+    if (R) {
+        if (R->rot < 0 || R->rot > C->HD || R->rot % 16 ||
+            (R->rot && (!R->table || !aligned16(R->table) || R->max_pos <= 0)) ||
+            (R->pairs != CPG_ROPE_HALVES && R->pairs != CPG_ROPE_ADJACENT)) {
+            cpg_set_error("cpg_paged_append: bad rotation (rot=%d, a multiple of 16 up to HD=%d; "
+                          "max_pos=%d; pairs=%d)", R->rot, C->HD, R->max_pos, R->pairs);
+            return -1;
+        }
+        if ((R->q_norm && !aligned16(R->q_norm)) || (R->k_norm && !aligned16(R->k_norm)) ||
+            ((R->q_norm || R->k_norm) && !(R->eps >= 0.0f && R->eps < INFINITY))) {
+            cpg_set_error("cpg_paged_append: bad head norm (gains on 16 bytes, eps=%g)", R->eps);
+            return -1;
+        }
+        a.table = R->table;
+        a.max_pos = R->max_pos;
+        a.rot = R->rot;
+        a.adjacent = R->pairs == CPG_ROPE_ADJACENT;
+        a.q_norm = R->q_norm;
+        a.k_norm = R->k_norm;
+        a.eps = R->eps;
+    }
+    if (check_ws("cpg_paged_append", ws, H ? H : ws ? ws->H : 0, C)) return -1;
+    CPG_REQUIRE_INIT();
+    if (B->S == 0 || B->T == 0) return 0;
+    a.q = q; a.k = k; a.v = v; a.q_out = q_out; a.kc = C->k; a.vc = C->v;
+    a.pages = B->pages; a.q_off = B->q_off; a.len = B->len;
+    a.ldq = ldq; a.ldk = ldk; a.ldv = ldv; a.ldqo = ldqo;
+    a.page_stride = C->page_stride; a.slot_stride = C->slot_stride; a.head_stride = C->head_stride;
+    a.H = H; a.KV = C->KV; a.HD = C->HD; a.S = B->S; a.T = B->T;
+    a.max_pages = B->max_pages; a.n_pages = C->n_pages; a.plog = log2_of(C->page);
+    a.stat = ws->stat;
+    const int gl = log2_of(C->HD / 8), hpw = 256 >> gl;
+    const dim3 grid(B->T, (H + 2 * C->KV + hpw - 1) / hpw);
+    auto kernel = type == CPG_T_F16    ? k_paged_append<CPG_T_F16, CPG_T_F16>
+                  : type == CPG_T_BF16 ? k_paged_append<CPG_T_BF16, CPG_T_BF16>
+                  : C->type == CPG_T_F32 ? k_paged_append<CPG_T_F32, CPG_T_F32>
+                  : C->type == CPG_T_F16 ? k_paged_append<CPG_T_F32, CPG_T_F16>
+                                         : k_paged_append<CPG_T_F32, CPG_T_BF16>;
+    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, g_cpg.stream, a, gl);
+    CPG_LAUNCH_CHECK("k_paged_append");
+    return 0;
+}
+
+extern "C" int cpg_paged_attn(const cpg_paged_cache *C, const cpg_paged_batch *B, int type, int H,
+                              const void *q, int64_t ldq, float scale, int window, void *out,
+                              int64_t ldo, float *lse, cpg_paged_ws *ws) {
+    if (check_call("cpg_paged_attn", C, B, type)) return -1;
+    if (H <= 0 || H % C->KV) { cpg_set_error("cpg_paged_attn: H=%d, KV=%d", H, C->KV); return -1; }
+    if (!(scale >= 0.0f && scale < INFINITY) || window < 0) {
+        cpg_set_error("cpg_paged_attn: scale %g, window %d (neither negative)", scale, window);
+        return -1;
+    }
+    if (!rows_ok(q, ldq, H, C->HD, type) || !rows_ok(out, ldo, H, C->HD, type)) {
+        cpg_set_error("cpg_paged_attn: rows of heads must not be null or overlap, and start on 16 bytes");
+        return -1;
+    }
+    if (check_ws("cpg_paged_attn", ws, H, C)) return -1;
+    CPG_REQUIRE_INIT();
+    if (B->S == 0 || B->T == 0) return 0;
+    pg_args a = {};
+    a.q = q; a.out = out; a.lse = lse; a.k = C->k; a.v = C->v; a.pages = B->pages;
+    a.ldq = ldq; a.ldo = ldo;
+    a.page_stride = C->page_stride; a.slot_stride = C->slot_stride; a.head_stride = C->head_stride;
+    a.H = H; a.G = H / C->KV; a.n_pages = C->n_pages;
+    a.scale2 = (scale > 0.0f ? scale : 1.0f / sqrtf((float)C->HD)) * 1.4426950408889634f;
+    a.zeros = ws->zeros; a.nans = ws->nans;
+    a.pacc = ws->pacc; a.pml = ws->pml; a.ctr = ws->ctr; a.stat = ws->stat;
+    const int rows = PG_FEW_ROWS;
+    a.hpp = a.G < rows ? a.G : rows;
+    a.b = pg_batch{B->q_off, B->len, B->S, B->T, C->KV, B->max_pages, log2_of(C->page),
+                   window < PG_MAX_LEN ? window : 0, (a.G + a.hpp - 1) / a.hpp, 0};
+    while ((2 << a.b.tl) * a.hpp <= rows) a.b.tl++;
+    /* no more workgroups than units there can be: tiles of the rows, and keys of a full page row */
+    const double tiles = (double)(B->T >> a.b.tl) + (B->S < B->T ? B->S : B->T);
+    const double units = tiles * C->KV * a.b.parts *
+                         ceil(ldexp((double)B->max_pages, a.b.plog) / PG_UNIT);
+    const int grid = units < PG_FEW_WGS ? (int)units : PG_FEW_WGS;
+    return pg_launch_few(a, type, C->type, C->HD, grid);
+}

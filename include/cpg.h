@@ -311,6 +311,97 @@ int cpg_gemv_norm(int enc, const void *w_tiled, int n_in, int n_out, const float
 /* out[t] = rmsnorm(x[t], g) (kernels.c:408-413; the sum of squares accumulated in double). */
 int cpg_rmsnorm(const float *x, const float *g, int T, int D, float eps, float *out);
 
+/* ---------------------------------------------------------------- paged key/value cache
+ * Keys and values of many sequences in pages of one pool, for programs that serve several
+ * conversations at once; no counterpart in the reference, whose cache is one conversation's.
+ * Two calls per layer and step, next to the projections (cpg_gemv_norm, cpg_gemv):
+ * cpg_paged_append takes the new tokens' heads in, cpg_paged_attn lets them attend.
+ *
+ * Element types of activations and cache. Activations f32 go with a cache of any of the three,
+ * f16 and bf16 with a cache of their own type. */
+#define CPG_T_F32  0
+#define CPG_T_F16  1
+#define CPG_T_BF16 2
+
+/* The pool: n_pages pages of `page` token slots (a power of two up to 1024). Element d of head h
+   of a page's slot is at page_id * page_stride + slot * slot_stride + h * head_stride + d of k and
+   of v, strides in elements; so (page, slot, head) and (page, head, slot) orders, a layer of a
+   pool of several and padded rows are all taken. HD is 64, 96, 128, 192 or 256. k, v and the
+   strides are multiples of 16 bytes. */
+typedef struct {
+    int KV, HD, type, page, n_pages;
+    int64_t page_stride, slot_stride, head_stride;
+    void *k, *v;                /* device */
+} cpg_paged_cache;
+
+/* The batch of a step: S sequences and the T rows of their new tokens. Rows q_off[s] ..
+   q_off[s+1] - 1 are sequence s's (q_off ascending, within 0 .. T; none is allowed), in the order
+   of their positions, which end at len[s] - 1: len[s] counts the tokens in the cache with the new
+   ones. Its token j lies in slot j % page of page pages[s * max_pages + j / page]. Rows that no
+   sequence has (behind q_off[S], as in a padded batch) are neither read nor written. The three
+   arrays are read on the device when the kernels run, so a captured graph can be replayed as the
+   batch moves on. T and each len are at most 2^30. max_new: about how many new tokens the longest sequence brings; it chooses
+   between kernels for few and for many tokens and is not relied on. */
+typedef struct {
+    int S, T, max_new, max_pages;
+    const int *pages, *q_off, *len;     /* device: (S, max_pages), (S + 1), (S) */
+} cpg_paged_batch;
+
+/* What cpg_paged_append does to query and key heads: RMSNorm of the head with gains q_norm and
+   k_norm (device (HD), NULL: none), then the rotation of the first `rot` elements (a multiple of
+   16 up to HD; 0: none) by the pairs of table row position: (max_pos, rot/2) (cos, sin) pairs, as
+   cpg_rope_table(theta, rot, max_pos, ...) writes them. Pair i is elements (i, i + rot/2)
+   (CPG_ROPE_HALVES, the model's own) or (2i, 2i + 1) (CPG_ROPE_ADJACENT). */
+#define CPG_ROPE_HALVES   0
+#define CPG_ROPE_ADJACENT 1
+typedef struct {
+    const float *table;         /* device */
+    int max_pos, rot, pairs;
+    const float *q_norm, *k_norm;
+    float eps;
+} cpg_paged_rope;
+
+/* Scratch for layers of H query heads, KV key/value heads and head_dim HD; one call at a time
+   per workspace (calls in stream order, and graphs replayed on the stream, are). */
+typedef struct cpg_paged_ws cpg_paged_ws;
+cpg_paged_ws *cpg_paged_ws_create(int H, int KV, int HD);
+void cpg_paged_ws_destroy(cpg_paged_ws *ws);
+/* Synchronises, then returns 1 when a call on ws since the last cpg_paged_ws_status met batch
+   data that it could not follow (and clears that), 0 when none did, negative on a device error.
+   Nothing outside the pool is touched for such data: q_off is taken within 0 .. T and ascending;
+   a sequence whose len is negative, beyond max_pages * page or beyond 2^30, a row whose position is negative or
+   beyond the rotation table, or a page id outside [0, n_pages) leaves the pool as it was, and
+   query rows of cpg_paged_append (not for a page id) and rows of cpg_paged_attn that depend on it
+   become NaN. (In cpg_paged_attn a row at a negative position has no key to see: zeros, not an
+   error.) */
+int cpg_paged_ws_status(cpg_paged_ws *ws);
+
+/* Row t's query heads q + t * ldq (H of HD), key heads k + t * ldk and value heads v + t * ldv (KV
+   of HD), all of `type`: queries and keys normed and rotated as R says (R NULL: as they are) at
+   the row's position; keys and values stored in the row's slot, rounded once to the cache's type,
+   and the queries written to q_out + t * ldqo in `type` (q_out may be q with ldqo = ldq). H = 0:
+   keys and values alone. ld in elements; pointers and rows multiples of 16 bytes. The arithmetic is
+   fp32. Two rows with the same slot (sequences that share a page they both write) race.
+   Asynchronous. */
+int cpg_paged_append(const cpg_paged_cache *C, const cpg_paged_batch *B, const cpg_paged_rope *R,
+                     int type, int H, const void *q, int64_t ldq, const void *k, int64_t ldk,
+                     const void *v, int64_t ldv, void *q_out, int64_t ldqo, cpg_paged_ws *ws);
+
+/* Attention of every row over its sequence's cached keys and values: query head h of the row at
+   position p attends with kv head h / (H / KV) over positions j <= p, and j > p - window where
+   window > 0: s_j = scale * q . k_j (scale > 0; 0: 1 / sqrt(HD)), out = softmax(s) . v at
+   out + t * ldo in `type`, and where lse is not NULL lse[t * H + h] = ln sum exp(s_j). A row with no
+   key to see gets zeros and lse -infinity. Keys and values that a row does not see do not reach
+   it, whatever they hold. Sums, softmax and accumulation are fp32; scores and weights are products
+   of f16 or bf16 matrix instructions: f32 activations in pieces that keep 22 or more bits of
+   them (from about 16 query rows per kv head on, an f32 cache too: keys and values beyond about
+   64000 become infinite there), 16-bit activations with the weights rounded to 16 bits. The way the
+   sums are split depends on the batch, and with it the last bits; the same call gives the same
+   bits. Asynchronous. */
+int cpg_paged_attn(const cpg_paged_cache *C, const cpg_paged_batch *B, int type, int H,
+                   const void *q, int64_t ldq, float scale, int window, void *out, int64_t ldo,
+                   float *lse, cpg_paged_ws *ws);
+
 /* ---------------------------------------------------------------- model glue
  * engine/api/cachepotato.c:108-166, :355-356 */
 /* out[t] = row ids[t] of a v4-layout table (rows x D; f32, Q8_0 or Q4_0), dequantised exactly;
