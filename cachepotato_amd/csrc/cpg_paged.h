@@ -9,22 +9,37 @@
 #define PG_FEW_ROWS 16      /* query rows of a tile of k_paged_few: one MFMA tile */
 #define PG_FEW_WGS 512      /* workgroups of k_paged_few at most: two per CU */
 
-/* one call of cpg_paged_attn, as the kernels get it */
+/* one call of cpg_paged_attn, as the kernels get it. Row offsets in the pool are taken in units of
+   2^ush bytes, the largest power of two that divides both strides, so that they fit 32 bits. */
 struct pg_args {
     const void *q;
+    const uint8_t *k, *v;
+    const int *pages;
+    pg_batch b;
+    int64_t ldq, head_bytes;
+    int H, G, n_pages, hpp; /* hpp: query heads per tile */
+    uint32_t page_units, slot_units;
+    int ush;
+    float scale2;           /* scale * log2(e) */
+    const uint8_t *blank;   /* 1 KiB of zeros, then 1 KiB of NaNs of every type: rows that are no key's */
+    /* ahead of here what the loop over the keys needs */
     void *out;
     float *lse;
-    const void *k, *v;
-    pg_batch b;
-    const int *pages;
-    int64_t ldq, ldo, page_stride, slot_stride, head_stride;
-    int H, G, n_pages, hpp; /* hpp: query heads per tile */
-    float scale2;           /* scale * log2(e) */
-    const void *zeros, *nans;
+    int64_t ldo;
     float *pacc;            /* partial results: (2 per workgroup) x rows x HD, and (M, l) of each row */
     float2 *pml;
     int *ctr, *stat;
 };
+/* The kernel's arguments read again where they are used: held in scalar registers over the loop,
+   the ones that only the end needs would be spilled. */
+__device__ static inline const pg_args *pg_late_args() {
+    auto p = __builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return (const pg_args *)p;
+}
+
+#define PG_NO_ROW 0xFFFFFFFFu   /* row offsets that are none: a key that no row sees, a bad page id */
+#define PG_BAD_ROW 0xFFFFFFFEu
 
 struct cpg_paged_ws {
     int H, KV, HD;
@@ -32,7 +47,7 @@ struct cpg_paged_ws {
     float *pacc;
     float2 *pml;
     int *ctr, *stat;
-    uint8_t *zeros, *nans;
+    uint8_t *blank;
     size_t rows;            /* partial rows there is room for */
 };
 
@@ -72,74 +87,66 @@ template <int TYPE> __device__ static inline void pg_put4(void *p, size_t i, flo
 
 /* ---------------------------------------------------------------- shares */
 
-__device__ static inline int64_t pg_wave_scan(int64_t v) {           /* inclusive */
+/* Where a share begins: the sequence of its first unit and the units before it there. Each
+   wavefront finds it by itself, without a barrier: lane l counts the units of sequences l c .. l c +
+   c - 1 (c = S / 64, rounded up), a scan over the lanes gives all units and the lane whose sequences
+   hold the first of the share, and those are gone through in the same way. stat: the workspace's
+   status word, set where the batch cannot be followed. */
+struct pg_start {
+    int s;
+    uint32_t rem;
+};
+
+__device__ static inline uint32_t pg_wave_scan(uint32_t v) {         /* inclusive */
     const int lane = threadIdx.x & 63;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
-        const int64_t p = __shfl_up(v, o);
-        if (lane >= o) v += p;
+        const uint32_t p = __shfl_up(v, o);
+        v += lane >= o ? p : 0;
     }
     return v;
 }
 
-/* The share of this workgroup. Every thread of the 256 calls it. sc: 8 words of LDS; stat: the
-   workspace's status word, set where the batch cannot be followed. */
-__device__ static inline pg_share pg_find_share(const pg_batch &b, int64_t *sc, int *stat) {
-    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
-    const int per = b.KV * b.parts;
+__device__ static inline pg_share pg_find_share(const pg_batch &b, pg_start &st, int *stat) {
+    const int lane = threadIdx.x & 63;
     auto units = [&](int s) {
-        if (s >= b.S) return (int64_t)0;
         const pg_seq q = pg_get_seq(b.q_off, b.len, s, b.T, b.max_pages, b.plog);
         if (blockIdx.x == 0 && q.bad && (q.cut || q.n > 0)) *stat = 1;
-        return q.n ? pg_units_before(q, b.tl, b.window, pg_tiles(q, b.tl)) * per : (int64_t)0;
+        return pg_seq_units(b, q);
     };
-    pg_share r;
-    r.s = 0;
+    st.s = 0;
     if (b.S == 1) {
-        r.U = units(0);
-        pg_deal(r, blockIdx.x, gridDim.x);
-        r.rem = r.u0;
+        const pg_share r = pg_deal(units(0), blockIdx.x, gridDim.x);
+        st.rem = r.u0;
         return r;
     }
-    /* one round of 256 sequences: the units before each of this thread's, and the round's sum */
-    auto round = [&](int s0, int64_t &before, int64_t &mine) {
-        mine = units(s0 + tid);
-        const int64_t inc = pg_wave_scan(mine);
-        __syncthreads();
-        if (lane == 63) sc[wv] = inc;
-        __syncthreads();
-        int64_t sum = 0, ahead = 0;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            ahead += i < wv ? sc[i] : 0;
-            sum += sc[i];
-        }
-        before = ahead + inc - mine;
-        return sum;
-    };
-    int64_t before, mine;
-    r.U = round(0, before, mine);
-    for (int s0 = 256; s0 < b.S; s0 += 256) {
-        int64_t b2, m2;
-        r.U += round(s0, b2, m2);
+    int first = 0, n = b.S, c = (n + 63) >> 6;   /* sequences [first, first + n) are looked at */
+    uint32_t mine = 0;
+    for (int i = 0; i < c; i++) {
+        const int s = lane * c + i;
+        mine += s < n ? units(s) : 0;
     }
-    pg_deal(r, blockIdx.x, gridDim.x);
-    __syncthreads();
-    int64_t base = 0;
-    for (int s0 = 0; s0 < b.S && base <= r.u0; s0 += 256) {
-        int64_t sum = 0;
-        if (b.S > 256) sum = round(s0, before, mine);
-        const int64_t at = base + before;
-        if (mine > 0 && at <= r.u0 && r.u0 < at + mine) {
-            sc[4] = s0 + tid;
-            sc[5] = r.u0 - at;
+    uint32_t inc = pg_wave_scan(mine);
+    const pg_share r = pg_deal(__builtin_amdgcn_readlane(inc, 63), blockIdx.x, gridDim.x);
+    st.rem = r.u0;
+    if (r.u0 == r.u1) return r;
+    for (;;) {
+        /* the first lane with the unit among its units or before them: lanes of no units are passed */
+        const uint64_t m = __ballot(inc > st.rem);
+        const int l = __ffsll((unsigned long long)m) - 1;
+        st.rem -= __builtin_amdgcn_readlane(inc - mine, l);
+        first += l * c;
+        if (c == 1) break;
+        n = min(c, first + c <= b.S ? c : b.S - first);
+        c = (n + 63) >> 6;
+        mine = 0;
+        for (int i = 0; i < c; i++) {
+            const int s = lane * c + i;
+            mine += s < n ? units(first + s) : 0;
         }
-        base += sum;
-        if (b.S <= 256) break;
+        inc = pg_wave_scan(mine);
     }
-    __syncthreads();
-    r.s = (int)sc[4];
-    r.rem = sc[5];
+    st.s = first;
     return r;
 }
 

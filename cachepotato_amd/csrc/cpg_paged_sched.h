@@ -5,7 +5,7 @@
  * kv head), and a tile's visible keys in units of UNIT. An item is one tile of one kv head (and of
  * one part of its query heads, where they are more than a tile's rows). The units of all items,
  * U of them in the order (sequence, kv head and part, tile, key), are dealt to W workgroups in equal
- * shares of neighbours: workgroup w takes units [w U / W, (w + 1) U / W). So a batch of one long
+ * shares of neighbours. So a batch of one long
  * and many short sequences keeps every workgroup as busy as one of equal lengths, with the lengths
  * known on the device alone. The price is a scan over the sequences ahead of the work, and items
  * cut by a border, whose pieces are merged by the last workgroup to arrive. */
@@ -19,15 +19,13 @@
 #define PG_FN static inline
 #endif
 
-#define PG_UL 7             /* log2 of the keys per unit of work */
-#define PG_UNIT (1 << PG_UL)
 #define PG_MAX_LEN (1 << 30) /* tokens of a sequence: positions and their sums stay in 32 bits */
 
-/* the batch and its division: S sequences, T rows; parts of a kv head's query heads, log2 of a
-   tile's tokens, log2 of a page's */
+/* the batch and its division: S sequences, T rows; parts of a kv head's query heads; log2 of the
+   tokens of a page, of those of a tile and of the keys of a unit (tl <= ul) */
 struct pg_batch {
     const int *q_off, *len;
-    int S, T, KV, max_pages, plog, window, parts, tl;
+    int S, T, KV, max_pages, plog, window, parts, tl, ul;
 };
 
 PG_FN int pg_min(int a, int b) { return a < b ? a : b; }
@@ -52,107 +50,106 @@ PG_FN pg_seq pg_get_seq(const int *q_off, const int *len,
     return r;
 }
 
-/* sum of floor(y / 2^k) over y < z */
-PG_FN int64_t pg_floor_sum(int z, int k) {
-    const int64_t q = z >> k, r = z & ((1 << k) - 1);
-    return ((q * (q - 1)) << k >> 1) + r * q;
+/* sum of floor(y / 2^k) over y < z, modulo 2^32 (differences of it are used) */
+PG_FN uint32_t pg_floor_sum(uint32_t z, int k) {
+    const uint32_t q = z >> k, r = z & ((1u << k) - 1);
+    return ((q & 1 ? q * ((q - 1) >> 1) : (q >> 1) * (q - 1)) << k) + r * q;
 }
 
-PG_FN int pg_tiles(const pg_seq &s, int tl) { return (s.n + (1 << tl) - 1) >> tl; }
+PG_FN int pg_tiles(const pg_seq &s, int tl) { return (int)(((uint32_t)s.n + (1u << tl) - 1) >> tl); }
 
-/* first and past-the-last unit of the keys that tile i sees; one empty unit where it sees none */
-PG_FN int pg_unit_lo(const pg_seq &s, int tl, int window, int i) {
-    return window > 0 ? pg_max(0, s.p0 + (i << tl) - window + 1) >> PG_UL : 0;
+/* first unit of the keys that tile i sees */
+PG_FN int pg_unit_lo(const pg_batch &b, const pg_seq &s, int i) {
+    return b.window > 0 ? pg_max(0, s.p0 + (i << b.tl) - b.window + 1) >> b.ul : 0;
 }
 
 /* units of the tiles before tile x of a sequence (every tile has one at least, so that the rows
    without a key are written too): with the position of a tile's last row a_i = p0 + (i + 1) TB - 1,
    the sum of floor(a_i / UNIT) + 1 - floor(b_i / UNIT) over the tiles with a key, b_i the first key
    that the tile's first row sees, in closed form since TB divides UNIT */
-PG_FN int64_t pg_units_before(const pg_seq &s, int tl, int window, int x) {
-    const int nt = pg_tiles(s, tl);
+PG_FN uint32_t pg_units_before(const pg_batch &b, const pg_seq &s, int x) {
+    const int nt = pg_tiles(s, b.tl), tl = b.tl;
     const int i0 = s.len <= 0 ? nt : s.p0 >= 0 ? 0 : (-s.p0) >> tl;   /* first tile with a key */
-    if (x <= i0) return x;
-    const int c = x - i0, k = PG_UL - tl;
+    if (x <= i0) return (uint32_t)x;
+    const int c = x - i0, k = b.ul - tl;
     const int A = (s.p0 + ((i0 + 1) << tl) - 1) >> tl;
-    int64_t sum = x + pg_floor_sum(A + c, k) - pg_floor_sum(A, k);
+    uint32_t sum = (uint32_t)x + pg_floor_sum(A + c, k) - pg_floor_sum(A, k);
     if (x == nt)                                 /* the last tile may be short */
-        sum += ((s.p0 + s.n - 1) >> PG_UL) - ((A + c - 1) >> k);
-    if (window > 0) {
-        const int64_t need = (int64_t)window - 1 - s.p0;              /* b_i >= 0 from here on */
-        const int64_t i1 = need <= 0 ? 0 : (need + (1 << tl) - 1) >> tl;
-        const int j = i1 > i0 ? (int)(i1 < x ? i1 : x) : i0;
+        sum += (uint32_t)(((s.p0 + s.n - 1) >> b.ul) - ((A + c - 1) >> k));
+    if (b.window > 0) {
+        const int need = b.window - 1 - s.p0;    /* b_i >= 0 from tile i1 on */
+        const int i1 = need <= 0 ? 0 : (int)(((uint32_t)need + (1u << tl) - 1) >> tl);
+        const int j = i1 > i0 ? pg_min(i1, x) : i0;
         if (j < x) {
-            const int B = (s.p0 + (j << tl) - window + 1) >> tl;
+            const int B = (s.p0 + (j << tl) - b.window + 1) >> tl;
             sum -= pg_floor_sum(B + x - j, k) - pg_floor_sum(B, k);
         }
     }
     return sum;
 }
 
-/* The share of a workgroup. Workgroups
-   beyond the number of units have none, so that between two that share an item every one has a
-   piece of it. Neighbours in the order of units are on one XCD where every workgroup has a share
-   (their tiles read the same keys; workgroup i of a launch runs on XCD i % 8), and spread over the
-   XCDs where not. */
+/* the units of a whole sequence, of all its kv heads and parts */
+PG_FN uint32_t pg_seq_units(const pg_batch &b, const pg_seq &s) {
+    return s.n ? pg_units_before(b, s, pg_tiles(s, b.tl)) * (uint32_t)(b.KV * b.parts) : 0;
+}
+
+/* The share of a workgroup: U / W units, one more for the first U % W. Workgroups beyond the number
+   of units have none, so that between two that share an item every one has a piece of it. Neighbours
+   in the order of units are on one XCD where every workgroup has a share (their tiles read the same
+   keys; workgroup i of a launch runs on XCD i % 8), and spread over the XCDs where not. */
 struct pg_share {
     int w, W;               /* this workgroup, of those that have a share */
-    int64_t U, u0, u1;      /* all units, and this workgroup's */
-    int s;                  /* the sequence of u0, and the units before u0 in it */
-    int64_t rem;
+    uint32_t U, u0, u1;     /* all units, and this workgroup's */
 };
 
-PG_FN void pg_deal(pg_share &r, int block, int grid) {
-    r.W = r.U < grid ? (int)r.U : grid;
+PG_FN pg_share pg_deal(uint32_t U, int block, int grid) {
+    pg_share r;
+    r.U = U;
+    r.W = U < (uint32_t)grid ? (int)U : grid;
     r.w = r.W < grid || grid % 8 ? block : block % 8 * (grid / 8) + block / 8;
-    const bool some = r.w < r.W;
-    r.u0 = some ? r.w * r.U / r.W : 0;
-    r.u1 = some ? (r.w + 1) * r.U / r.W : 0;
+    r.u0 = r.u1 = 0;
+    if (r.w < r.W) {
+        const uint32_t per = U / (uint32_t)r.W, more = U - per * r.W, w = (uint32_t)r.w;
+        r.u0 = w * per + (w < more ? w : more);
+        r.u1 = r.u0 + per + (w < more);
+    }
+    return r;
 }
 
 /* the workgroup that has unit u */
-PG_FN int pg_owner(int64_t u, int64_t U, int W) { return (int)(((u + 1) * W - 1) / U); }
+PG_FN int pg_owner(uint32_t u, uint32_t U, int W) {
+    const uint32_t per = U / (uint32_t)W, more = U - per * W, wide = more * (per + 1);
+    return (int)(u < wide ? u / (per + 1) : more + (u - wide) / per);
+}
 
 /* a walk over a share's items */
 struct pg_item {
-    pg_seq q;
-    int s, kv, part, tile;  /* the item */
+    int kv, part, tile;     /* the item */
     int off, cnt;           /* its units from `off` on, cnt of them, are this workgroup's */
     int all;                /* its units */
-    int64_t first;          /* the number of its first unit among all */
+    uint32_t first;         /* the number of its first unit among all */
 };
 
-/* the item at unit u (u0 <= u < u1) of the share; s and rem are moved on past it */
-PG_FN pg_item pg_next_item(const pg_batch &b, int64_t u, int64_t u1, int &s,
-                                              int64_t &rem) {
+/* the item of sequence q at unit u (below u1, `rem` units into the sequence) */
+PG_FN pg_item pg_find_item(const pg_batch &b, const pg_seq &q, uint32_t u, uint32_t u1, uint32_t rem) {
     pg_item it;
-    int64_t per;
-    for (;;) {
-        it.q = pg_get_seq(b.q_off, b.len, s, b.T, b.max_pages, b.plog);
-        per = it.q.n ? pg_units_before(it.q, b.tl, b.window, pg_tiles(it.q, b.tl)) : 0;
-        if (rem < per * b.KV * b.parts || s + 1 >= b.S) break;
-        s++;
-        rem = 0;
-    }
-    it.s = s;
-    const uint32_t kp = (uint32_t)(rem / per);
-    const int64_t in = rem - kp * per;
-    it.kv = kp / b.parts;
-    it.part = kp % b.parts;
-    int lo = 0, hi = pg_tiles(it.q, b.tl);       /* the tile: units_before(lo) <= in < units_before(hi) */
+    const int nt = pg_tiles(q, b.tl);
+    const uint32_t per = pg_units_before(b, q, nt), kp = rem / per, in = rem - kp * per;
+    it.kv = b.parts == 1 ? (int)kp : (int)(kp / (uint32_t)b.parts);
+    it.part = (int)kp - it.kv * b.parts;
+    uint32_t ahead = 0, upto = per;
+    int lo = 0, hi = nt;                         /* units_before(lo) <= in < units_before(hi) */
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        if (pg_units_before(it.q, b.tl, b.window, mid) <= in) lo = mid;
-        else hi = mid;
+        const uint32_t x = pg_units_before(b, q, mid);
+        if (x <= in) { lo = mid; ahead = x; }
+        else { hi = mid; upto = x; }
     }
     it.tile = lo;
-    const int64_t ahead = pg_units_before(it.q, b.tl, b.window, lo);
-    it.all = (int)(pg_units_before(it.q, b.tl, b.window, lo + 1) - ahead);
+    it.all = (int)(upto - ahead);
     it.off = (int)(in - ahead);
     it.first = u - it.off;
-    const int64_t left = u1 - u;
-    it.cnt = it.all - it.off < left ? it.all - it.off : (int)left;
-    rem += it.cnt;
+    it.cnt = pg_min(it.all - it.off, (int)(u1 - u));
     return it;
 }
 

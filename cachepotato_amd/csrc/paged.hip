@@ -164,6 +164,14 @@ static bool rows_ok(const void *p, int64_t ld, int heads, int HD, int type) {
     return p && aligned16(p) && ld >= (int64_t)heads * HD && ld * elem_bytes(type) % 16 == 0;
 }
 
+/* log2 of the largest power of two of bytes that divides both strides of a slot's offset in the pool */
+static int row_shift(const cpg_paged_cache *C) {
+    const int64_t all = (C->n_pages > 1 ? C->page_stride : 0) | (C->page > 1 ? C->slot_stride : 0);
+    int s = 4;
+    while (s < 20 && !(all * elem_bytes(C->type) >> s & 1)) s++;
+    return s;
+}
+
 /* the checks that both entry points make, of the arguments and then of the workspace; 0, or -1
    with the reason set */
 static int check_call(const char *who, const cpg_paged_cache *C, const cpg_paged_batch *B, int type) {
@@ -194,11 +202,18 @@ static int check_call(const char *who, const cpg_paged_cache *C, const cpg_paged
             return -1;
         }
     }
+    /* slots are found at 32-bit offsets in units of row_shift: at least 64 GiB, 1 TiB for strides of
+       256 bytes */
+    const double last = ((double)(C->n_pages - 1) * (n[0] > 1 ? st[0] : 0) + (double)(C->page - 1) * (n[1] > 1 ? st[1] : 0)) * eb;
+    if (ldexp(last, -row_shift(C)) >= 4294967040.0) {
+        cpg_set_error("%s: a pool of %.0f bytes is too large for its strides", who, last);
+        return -1;
+    }
     if (!aligned16(C->k) || !aligned16(C->v)) {
         cpg_set_error("%s: the pool is not aligned to 16 bytes", who);
         return -1;
     }
-    if (B->S < 0 || B->T < 0 || B->T > PG_MAX_LEN || B->max_pages < 0 ||
+    if (B->S < 0 || B->S > PG_MAX_LEN || B->T < 0 || B->T > PG_MAX_LEN || B->max_pages < 0 ||
         (B->S > 0 && B->T > 0 && (!B->q_off || !B->len || !B->pages || B->max_pages == 0))) {
         cpg_set_error("%s: bad batch S=%d T=%d max_pages=%d", who, B->S, B->T, B->max_pages);
         return -1;
@@ -237,21 +252,21 @@ extern "C" cpg_paged_ws *cpg_paged_ws_create(int H, int KV, int HD) {
     ws->KV = KV;
     ws->HD = HD;
     ws->rows = (size_t)2 * PG_FEW_WGS * PG_FEW_ROWS;
-    const size_t sz[6] = {ws->rows * HD * 4, ws->rows * 8, PG_FEW_WGS * 4, 4, 1024, 1024};
+    const size_t sz[5] = {ws->rows * HD * 4, ws->rows * 8, (size_t)3 * PG_FEW_WGS * 4, 4, 2048};
     size_t total = 0;
-    for (int i = 0; i < 6; i++) total += cpg_round256(sz[i]);
+    for (int i = 0; i < 5; i++) total += cpg_round256(sz[i]);
     uint8_t *p = (uint8_t *)cpg_malloc(total);
     if (!p) { free(ws); return nullptr; }
     ws->block = p;
-    void **dst[6] = {(void **)&ws->pacc, (void **)&ws->pml, (void **)&ws->ctr, (void **)&ws->stat,
-                     (void **)&ws->zeros, (void **)&ws->nans};
-    for (int i = 0; i < 6; i++) {
+    void **dst[5] = {(void **)&ws->pacc, (void **)&ws->pml, (void **)&ws->ctr, (void **)&ws->stat,
+                     (void **)&ws->blank};
+    for (int i = 0; i < 5; i++) {
         *dst[i] = p;
         p += cpg_round256(sz[i]);
     }
-    /* nans: every bit set is a NaN in all three element types */
+    /* every bit set is a NaN in all three element types */
     if (cpg_memset(ws->ctr, 0, sz[2]) || cpg_memset(ws->stat, 0, 4) ||
-        cpg_memset(ws->zeros, 0, 1024) || cpg_memset(ws->nans, 255, 1024)) {
+        cpg_memset(ws->blank, 0, 1024) || cpg_memset(ws->blank + 1024, 255, 1024)) {
         cpg_paged_ws_destroy(ws);
         return nullptr;
     }
@@ -345,22 +360,36 @@ extern "C" int cpg_paged_attn(const cpg_paged_cache *C, const cpg_paged_batch *B
     CPG_REQUIRE_INIT();
     if (B->S == 0 || B->T == 0) return 0;
     pg_args a = {};
-    a.q = q; a.out = out; a.lse = lse; a.k = C->k; a.v = C->v; a.pages = B->pages;
-    a.ldq = ldq; a.ldo = ldo;
-    a.page_stride = C->page_stride; a.slot_stride = C->slot_stride; a.head_stride = C->head_stride;
+    const int eb = elem_bytes(C->type);
+    a.q = q; a.out = out; a.lse = lse; a.pages = B->pages;
+    a.k = (const uint8_t *)C->k; a.v = (const uint8_t *)C->v;
+    a.ldq = ldq; a.ldo = ldo; a.head_bytes = C->head_stride * eb;
     a.H = H; a.G = H / C->KV; a.n_pages = C->n_pages;
+    a.ush = row_shift(C);
+    a.page_units = (uint32_t)(C->page_stride * eb >> a.ush);
+    a.slot_units = (uint32_t)(C->slot_stride * eb >> a.ush);
     a.scale2 = (scale > 0.0f ? scale : 1.0f / sqrtf((float)C->HD)) * 1.4426950408889634f;
-    a.zeros = ws->zeros; a.nans = ws->nans;
+    a.blank = ws->blank;
     a.pacc = ws->pacc; a.pml = ws->pml; a.ctr = ws->ctr; a.stat = ws->stat;
     const int rows = PG_FEW_ROWS;
     a.hpp = a.G < rows ? a.G : rows;
+    /* a unit is one step of a workgroup's four wavefronts: 64 keys of an f32 cache, 128 of a 16-bit
+       one (more where the units of the largest batch there can be would not fit 31 bits) */
     a.b = pg_batch{B->q_off, B->len, B->S, B->T, C->KV, B->max_pages, log2_of(C->page),
-                   window < PG_MAX_LEN ? window : 0, (a.G + a.hpp - 1) / a.hpp, 0};
+                   window < PG_MAX_LEN ? window : 0, (a.G + a.hpp - 1) / a.hpp, 0,
+                   C->type == CPG_T_F32 ? 6 : 7};
     while ((2 << a.b.tl) * a.hpp <= rows) a.b.tl++;
     /* no more workgroups than units there can be: tiles of the rows, and keys of a full page row */
     const double tiles = (double)(B->T >> a.b.tl) + (B->S < B->T ? B->S : B->T);
-    const double units = tiles * C->KV * a.b.parts *
-                         ceil(ldexp((double)B->max_pages, a.b.plog) / PG_UNIT);
+    double units;
+    for (;; a.b.ul++) {
+        units = tiles * C->KV * a.b.parts * ceil(ldexp((double)B->max_pages, a.b.plog - a.b.ul));
+        if (units < 2147483648.0 || a.b.ul >= 30) break;
+    }
+    if (units >= 2147483648.0) {
+        cpg_set_error("cpg_paged_attn: a batch of %d rows and %d sequences of %d heads is too large", B->T, B->S, H);
+        return -1;
+    }
     const int grid = units < PG_FEW_WGS ? (int)units : PG_FEW_WGS;
     return pg_launch_few(a, type, C->type, C->HD, grid);
 }

@@ -77,33 +77,43 @@ template <int CT, int HD> struct pg_buf {
     uint32_t v[NR][NW];
 };
 
-template <int NW> __device__ static inline void pg_load_words(const uint8_t *p, uint32_t (&w)[NW]) {
+/* An address computed as a number, for loads from global memory: as a generic pointer its loads
+   would count as LDS operations too, and every LDS read would wait for all of them. */
+template <typename T> __device__ static inline T pg_load(uint64_t p) {
+    return *(const __attribute__((address_space(1))) T *)p;
+}
+
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+
+template <int NW> __device__ static inline void pg_load_words(uint64_t p, uint32_t (&w)[NW]) {
     /* the lane's part of a row starts on a multiple of 4 NW bytes of it */
     if constexpr (NW % 4 == 0) {
 #pragma unroll
         for (int i = 0; i < NW / 4; i++) {
-            const uint4 u = ((const uint4 *)p)[i];
+            const u32x4_t u = pg_load<u32x4_t>(p + 16 * i);
             w[4 * i] = u.x; w[4 * i + 1] = u.y; w[4 * i + 2] = u.z; w[4 * i + 3] = u.w;
         }
     } else if constexpr (NW % 2 == 0) {
 #pragma unroll
         for (int i = 0; i < NW / 2; i++) {
-            const uint2 u = ((const uint2 *)p)[i];
+            const u32x2_t u = pg_load<u32x2_t>(p + 8 * i);
             w[2 * i] = u.x; w[2 * i + 1] = u.y;
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < NW; i++) w[i] = ((const uint32_t *)p)[i];
+        for (int i = 0; i < NW; i++) w[i] = pg_load<uint32_t>(p + 4 * i);
     }
 }
 
-/* one word with an infinity or a NaN in it */
-template <int CT> __device__ static inline bool pg_wild(uint32_t w) {
-    if constexpr (CT == CPG_T_F32) return (w & 0x7F800000u) == 0x7F800000u;
-    constexpr uint32_t E = CT == CPG_T_F16 ? 0x7C00u : 0x7F80u;
-    return (w & E) == E || (w >> 16 & E) == E;
+/* the top bit of a word (of both its halves, for 16-bit types) set where the exponent is all ones,
+   an infinity's or a NaN's: one step more carries into it. Words, not truth values, which would
+   fill the scalar registers. */
+template <int CT> __device__ static inline uint32_t pg_wild(uint32_t w) {
+    constexpr uint32_t E = CT == CPG_T_F32 ? 0x7F800000u : CT == CPG_T_F16 ? 0x7C007C00u : 0x7F807F80u;
+    constexpr uint32_t ONE = CT == CPG_T_F32 ? 0x00800000u : CT == CPG_T_F16 ? 0x04000400u : 0x00800080u;
+    return ((w & E) + ONE) & (CT == CPG_T_F32 ? 0x80000000u : 0x80008000u);
 }
-
 /* grid W workgroups of 256 threads, each with its share of the units (cpg_paged.h) */
 template <int CT, int AT, int HD>
 __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_paged_few(const pg_args a) {
@@ -114,275 +124,288 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_paged_few(const pg_a
     constexpr int EB = F32 ? 4 : 2, NS = F32 ? HD / 16 : HD / 32, LD = HD + 4;
     __shared__ __align__(16) float o_s[4][16][LD];
     __shared__ float m_s[4][16], l_s[4][16];
-    __shared__ int64_t sc[8];
     __shared__ int flag;
-    const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
-    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const pg_share sh = pg_find_share(a.b, sc, a.stat);
+    const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    pg_start at;
+    const pg_share sh = pg_find_share(a.b, at, a.stat);
     const int W = sh.W, me = sh.w;
-    int s = sh.s;
-    int64_t rem = sh.rem;
-    for (int64_t u = sh.u0; u < sh.u1;) {
-        const pg_item it = pg_next_item(a.b, u, sh.u1, s, rem);
+    int s = at.s;
+    uint32_t rem = at.rem;
+    for (uint32_t u = sh.u0; u < sh.u1;) {
+        const pg_seq sq = pg_get_seq(a.b.q_off, a.b.len, s, a.b.T, a.b.max_pages, a.b.plog);
+        if (rem >= pg_seq_units(a.b, sq)) {      /* the sequence is done, or brings nothing */
+            s++;
+            rem = 0;
+            continue;
+        }
+        const pg_item it = pg_find_item(a.b, sq, u, sh.u1, rem);
         u += it.cnt;
+        rem += it.cnt;
+        /* the thread's number is made opaque, here and behind the loop: what follows from it would
+           else be computed ahead of the walk and held, or spilled, over everything */
+        int lane = tid & 63;
+        asm volatile("" : "+v"(lane));
+        const int c = lane & 15, g = lane >> 4;
         /* the lane's query: row c of the tile */
-        const int t0 = it.tile << a.b.tl, tb = min(1 << a.b.tl, it.q.n - t0);
+        const int t0 = it.tile << a.b.tl, tb = min(1 << a.b.tl, sq.n - t0);
         const int tok = c / a.hpp, hq = it.part * a.hpp + c - tok * a.hpp;
         const bool row_ok = tok < tb && hq < a.G;
-        const int pos = row_ok ? it.q.p0 + t0 + tok : -1;           /* keys pos_lo .. pos */
+        const int pos = row_ok ? sq.p0 + t0 + tok : -1;           /* keys pos_lo .. pos */
         const int pos_lo = a.b.window > 0 ? max(0, pos - a.b.window + 1) : 0;
-        const size_t qrow = (size_t)(it.q.lo + t0 + min(tok, tb - 1));
+        const size_t qrow = (size_t)(sq.lo + t0 + min(tok, tb - 1));
         const int qh = it.kv * a.G + min(hq, a.G - 1);
-        const int first = it.q.p0 + t0, last = first + tb - 1;      /* positions of the tile */
+        const int first = sq.p0 + t0, last = first + tb - 1;      /* positions of the tile */
         const int klo = a.b.window > 0 ? max(0, first - a.b.window + 1) : 0, khi = last + 1;
         const int full_lo = a.b.window > 0 ? max(0, last - a.b.window + 1) : 0;
         /* the units' keys */
-        const int j0 = (pg_unit_lo(it.q, a.b.tl, a.b.window, it.tile) + it.off) << PG_UL;
-        const int jend = min(j0 + (it.cnt << PG_UL), khi);
+        const int j0 = (pg_unit_lo(a.b, sq, it.tile) + it.off) << a.b.ul;
+        const int jend = (int)min((int64_t)j0 + ((int64_t)it.cnt << a.b.ul), (int64_t)khi);
         f32x4_t o[DPL];
 #pragma unroll
         for (int j = 0; j < DPL; j++) o[j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
         float m = -INFINITY, M = 0.0f, l = 0.0f;
-        if (it.q.len > 0 && jend > j0) {
-            /* ---- the queries, in the order the key rows are loaded in */
-            uint4 qf[NP][NS];
-            float cs = a.scale2;
-            {
-                const size_t e = qrow * a.ldq + (size_t)qh * HD;
-                if constexpr (F32) {
-                    const float *qp = (const float *)a.q + e + 4 * g;
+        /* no branch around the loads, also where the tile sees no key: what its two sides bring would
+           be joined in registers of their own */
+        const int *ids = a.pages + (size_t)s * a.b.max_pages;
+        const int pmask = (1 << a.b.plog) - 1;
+        const uint8_t *kb = a.k + (size_t)it.kv * a.head_bytes;
+        const uint8_t *vb = a.v + (size_t)it.kv * a.head_bytes;
+        /* step n of this wavefront: keys jw + 4 KT n .. + KT - 1 */
+        const int jw = j0 + KT * w;
+        const int steps = jend > jw ? (jend - jw + 4 * KT - 1) / (4 * KT) : 0;
+        /* the page of the step's key lane % KT (of a key that no row sees: any that one does) */
+        auto page_of = [&](int n) __attribute__((always_inline)) {
+            const int j = jw + 4 * KT * n + lane % KT;
+            return ids[max(min(max(j, klo), khi - 1), 0) >> a.b.plog];
+        };
+        /* its row's offset. A key that no row sees reads zeros; a page id that is none makes the
+           key NaN, and with it every score of it */
+        auto row_of = [&](int n, int id) __attribute__((always_inline)) {
+            const int j = jw + 4 * KT * n + lane % KT;
+            const bool out = j < klo || j >= khi, miss = (uint32_t)id >= (uint32_t)a.n_pages;
+            if (__any(miss && !out) && lane == 0) *pg_late_args()->stat = 1;
+            const uint32_t r = (uint32_t)id * a.page_units + (uint32_t)(j & pmask) * a.slot_units;
+            return out ? PG_NO_ROW : miss ? PG_BAD_ROW : r;
+        };
+        auto row_ptr = [&](const uint8_t *base, uint32_t r, bool key) __attribute__((always_inline)) {
+            const uint64_t p = (uint64_t)base + ((uint64_t)r << a.ush);
+            const uint64_t no = (uint64_t)a.blank + (key && r == PG_BAD_ROW ? 1024 : 0);
+            return r >= PG_BAD_ROW ? no : p;
+        };
+        buf b;
+        auto load_k = [&](uint32_t ro) __attribute__((always_inline)) {
 #pragma unroll
-                    for (int i = 0; i < NS; i++) qf[0][i] = *(const uint4 *)(qp + 16 * i);
-                } else if constexpr (AT != CPG_T_F32) {
-                    const uint16_t *qp = (const uint16_t *)a.q + e + 8 * g;
+            for (int t = 0; t < KT / 16; t++) {
+                const uint64_t p = row_ptr(kb, __shfl(ro, 16 * t + c), true) + 16 * g;
 #pragma unroll
-                    for (int i = 0; i < NS; i++) qf[0][i] = *(const uint4 *)(qp + 32 * i);
-                } else {
-                    const float *qp = (const float *)a.q + e + 8 * g;
-                    float x[NS][8], top = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < NS; i++) {
-                        const float4 u0 = *(const float4 *)(qp + 32 * i), u1 = *(const float4 *)(qp + 32 * i + 4);
-                        x[i][0] = u0.x; x[i][1] = u0.y; x[i][2] = u0.z; x[i][3] = u0.w;
-                        x[i][4] = u1.x; x[i][5] = u1.y; x[i][6] = u1.z; x[i][7] = u1.w;
-#pragma unroll
-                        for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(x[i][j]));
-                    }
-                    top = fmaxf(top, __shfl_xor(top, 16));
-                    top = fmaxf(top, __shfl_xor(top, 32));
-                    /* the row by 2^-ex, its largest element in [0.5, 1), and the scores by 2^ex */
-                    const int ex = top > 0.0f && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) : 0;
-                    cs = ldexpf(cs, ex);
-#pragma unroll
-                    for (int i = 0; i < NS; i++) {
-                        uint32_t wd[4][NP];
-#pragma unroll
-                        for (int j = 0; j < 4; j++)
-                            pg_pieces2<CT, NP>(ldexpf(x[i][2 * j], -ex), ldexpf(x[i][2 * j + 1], -ex), wd[j]);
-#pragma unroll
-                        for (int n = 0; n < NP; n++) qf[n][i] = make_uint4(wd[0][n], wd[1][n], wd[2][n], wd[3][n]);
-                    }
-                }
-                if (!row_ok)
-#pragma unroll
-                    for (int n = 0; n < NP; n++)
-#pragma unroll
-                        for (int i = 0; i < NS; i++) qf[n][i] = make_uint4(0, 0, 0, 0);
+                for (int i = 0; i < NS; i++) b.k[t * NS + i] = __builtin_bit_cast(uint4, pg_load<u32x4_t>(p + 64 * i));
             }
-            const int *ids = a.pages + (size_t)it.s * a.b.max_pages;
-            const int pmask = (1 << a.b.plog) - 1;
-            const uint8_t *kb = (const uint8_t *)a.k + (size_t)it.kv * a.head_stride * EB;
-            const uint8_t *vb = (const uint8_t *)a.v + (size_t)it.kv * a.head_stride * EB;
-            /* step n of this wavefront: keys jw + 4 KT n .. + KT - 1 */
-            const int jw = j0 + KT * w;
-            const int steps = jend > jw ? (jend - jw + 4 * KT - 1) / (4 * KT) : 0;
-            /* the page of the step's key lane % KT (a key that no row sees: any that one does) */
-            auto page_of = [&](int n) __attribute__((always_inline)) {
-                const int j = jw + 4 * KT * n + lane % KT;
-                return ids[min(max(j, klo), khi - 1) >> a.b.plog];
-            };
-            /* its key and value rows. A key that no row sees reads zeros; a page id that is none
-               makes the key NaN, and with it every score of it */
-            buf b;
-            auto where = [&](int n, int i, int id, bool &out, bool &miss) __attribute__((always_inline)) {
-                const int j = jw + 4 * KT * n + i, p = __shfl(id, i);
-                out = j < klo || j >= khi;
-                miss = p < 0 || p >= a.n_pages;
-                return ((size_t)(miss ? 0 : p) * a.page_stride + (size_t)(j & pmask) * a.slot_stride) * EB;
-            };
-            auto load_k = [&](int n, int id) __attribute__((always_inline)) {
+        };
+        auto load_v = [&](uint32_t ro) __attribute__((always_inline)) {
 #pragma unroll
-                for (int t = 0; t < KT / 16; t++) {
-                    bool out, miss;
-                    const size_t off = where(n, 16 * t + c, id, out, miss);
-                    const uint8_t *p = out ? (const uint8_t *)a.zeros : miss ? (const uint8_t *)a.nans : kb + off;
-                    p += 16 * g;
+            for (int r = 0; r < NR; r++)
+                pg_load_words<NW>(row_ptr(vb, __shfl(ro, 16 * (r >> 2) + 4 * g + (r & 3)), false) + c * DPL * EB, b.v[r]);
+        };
+        int id = page_of(0);
+        /* ---- the queries, in the order the key rows are loaded in; issued between the first
+           page ids and the first keys, and put into pieces while those fly */
+        constexpr int QN = F32 || AT != CPG_T_F32 ? NS : 2 * NS;
+        const uint8_t *qp = (const uint8_t *)a.q +
+                            (qrow * a.ldq + (size_t)qh * HD) * (AT == CPG_T_F32 ? 4 : 2) +
+                            g * (QN == 2 * NS ? 32 : 16);
+        uint4 qraw[QN];
 #pragma unroll
-                    for (int i = 0; i < buf::NK / (KT / 16); i++)
-                        b.k[t * (buf::NK / (KT / 16)) + i] = *(const uint4 *)(p + 64 * i);
-                }
-                if (__any(id < 0 || id >= a.n_pages) && lane == 0) *a.stat = 1;
-            };
-            auto load_v = [&](int n, int id) __attribute__((always_inline)) {
+        for (int i = 0; i < QN; i++)
+            qraw[i] = *(const uint4 *)(qp + (QN == NS ? 64 * i : 128 * (i >> 1) + 16 * (i & 1)));
+        __builtin_amdgcn_sched_barrier(0);
+        uint32_t ro = row_of(0, id);
+        id = page_of(1);                     /* ahead of the loads, so that it is there with them */
+        load_k(ro);
+        load_v(ro);
+        __builtin_amdgcn_sched_barrier(0);
+        uint4 qf[NP][NS];
+        float cs = a.scale2;
+        if constexpr (QN == NS) {
 #pragma unroll
-                for (int r = 0; r < NR; r++) {
-                    bool out, miss;
-                    const size_t off = where(n, 16 * (r >> 2) + 4 * g + (r & 3), id, out, miss);
-                    const uint8_t *p = out || miss ? (const uint8_t *)a.zeros : vb + off;
-                    pg_load_words<NW>(p + c * DPL * EB, b.v[r]);
-                }
-            };
-            int id = 0;
-            if (steps > 0) {
-                id = page_of(0);
-                load_k(0, id);
-                load_v(0, id);
-                id = page_of(1);
+            for (int i = 0; i < NS; i++) qf[0][i] = row_ok ? qraw[i] : make_uint4(0, 0, 0, 0);
+        } else {
+            float top = 0.0f;
+#pragma unroll
+            for (int i = 0; i < QN; i++) {
+                const uint32_t x[4] = {qraw[i].x, qraw[i].y, qraw[i].z, qraw[i].w};
+#pragma unroll
+                for (int j = 0; j < 4; j++) top = fmaxf(top, fabsf(__uint_as_float(x[j])));
             }
-            for (int n = 0; n < steps; n++) {
-                const int jb = jw + 4 * KT * n;
-                /* scores: st[t][i] of key jb + 16 t + 4 g + i */
-                f32x4_t st[KT / 16];
+            top = fmaxf(top, __shfl_xor(top, 16));
+            top = fmaxf(top, __shfl_xor(top, 32));
+            /* the row by 2^-ex, its largest element in [0.5, 1), and the scores by 2^ex */
+            const int ex = top > 0.0f && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) : 0;
+            cs = ldexpf(cs, ex);
 #pragma unroll
-                for (int t = 0; t < KT / 16; t++) {
-                    st[t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int i = 0; i < NS; i++) {
+                const uint4 r0 = qraw[2 * i], r1 = qraw[2 * i + 1];
+                const uint32_t x[8] = {r0.x, r0.y, r0.z, r0.w, r1.x, r1.y, r1.z, r1.w};
+                uint32_t wd[4][NP];
 #pragma unroll
-                    for (int i = 0; i < NS; i++) {
-                        const uint4 kf = b.k[t * NS + i];
-                        if constexpr (F32) {
-                            const uint4 qv = qf[0][i];
-                            st[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kf.x), __uint_as_float(qv.x), st[t], 0, 0, 0);
-                            st[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kf.y), __uint_as_float(qv.y), st[t], 0, 0, 0);
-                            st[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kf.z), __uint_as_float(qv.z), st[t], 0, 0, 0);
-                            st[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kf.w), __uint_as_float(qv.w), st[t], 0, 0, 0);
-                        } else {
+                for (int j = 0; j < 4; j++)
+                    pg_pieces2<CT, NP>(ldexpf(__uint_as_float(x[2 * j]), -ex),
+                                       ldexpf(__uint_as_float(x[2 * j + 1]), -ex), wd[j]);
 #pragma unroll
-                            for (int p = NP - 1; p >= 0; p--) st[t] = pg_mfma16<CT>(kf, qf[p][i], st[t]);
-                        }
+                for (int n = 0; n < NP; n++)
+                    qf[n][i] = row_ok ? make_uint4(wd[0][n], wd[1][n], wd[2][n], wd[3][n]) : make_uint4(0, 0, 0, 0);
+            }
+        }
+        for (int n = 0; n < steps; n++) {
+            const int jb = jw + 4 * KT * n;
+            /* scores: st[t][i] of key jb + 16 t + 4 g + i */
+            f32x4_t st[KT / 16];
+#pragma unroll
+            for (int t = 0; t < KT / 16; t++) {
+                st[t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int i = 0; i < NS; i++) {
+                    const uint4 kf = b.k[t * NS + i];
+                    if constexpr (F32) {
+                        const uint4 qv = qf[0][i];
+                        st[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kf.x), __uint_as_float(qv.x), st[t], 0, 0, 0);
+                        st[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kf.y), __uint_as_float(qv.y), st[t], 0, 0, 0);
+                        st[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kf.z), __uint_as_float(qv.z), st[t], 0, 0, 0);
+                        st[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kf.w), __uint_as_float(qv.w), st[t], 0, 0, 0);
+                    } else {
+#pragma unroll
+                        for (int p = NP - 1; p >= 0; p--) st[t] = pg_mfma16<CT>(kf, qf[p][i], st[t]);
                     }
                 }
-                /* the key registers are free: without the fence the loads would be moved ahead of
-                   the scores, into registers of their own */
-                __builtin_amdgcn_sched_barrier(0);
-                load_k(n + 1, id);               /* past the last step: zeros */
-                __builtin_amdgcn_sched_barrier(0);
-                const bool edge = jb < full_lo || jb + KT - 1 > first;
-                if (edge)                        /* some row does not see some key */
-#pragma unroll
-                    for (int t = 0; t < KT / 16; t++)
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const int j = jb + 16 * t + 4 * g + i;
-                            st[t][i] = j <= pos && j >= pos_lo ? st[t][i] : -INFINITY;
-                        }
-                float mn = m;
+            }
+            /* the key registers are free: without the fence the loads would be moved ahead of
+               the scores, into registers of their own */
+            __builtin_amdgcn_sched_barrier(0);
+            ro = row_of(n + 1, id);          /* past the last step: zeros */
+            id = page_of(n + 2);
+            load_k(ro);
+            __builtin_amdgcn_sched_barrier(0);
+            const bool edge = jb < full_lo || jb + KT - 1 > first;
+            if (edge)                        /* some row does not see some key */
 #pragma unroll
                 for (int t = 0; t < KT / 16; t++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) mn = fmaxf(mn, st[t][i]);
-                mn = fmaxf(mn, __shfl_xor(mn, 16));
-                mn = fmaxf(mn, __shfl_xor(mn, 32));
-                if (__any(mn > m)) {
-                    const float Mn = mn == -INFINITY ? 0.0f : cs * mn;
-                    const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - Mn);
-                    m = mn;
-                    M = Mn;
-                    l *= f;
-#pragma unroll
-                    for (int j = 0; j < DPL; j++)
-#pragma unroll
-                        for (int i = 0; i < 4; i++) o[j][i] *= f;
-                }
-                float p[NR];
-#pragma unroll
-                for (int r = 0; r < NR; r++) {
-                    p[r] = __builtin_amdgcn_exp2f(fmaf(st[r >> 2][r & 3], cs, P::LIFT - M));
-                    l += p[r];
-                }
-                /* values that some row does not see and that are no numbers: taken row by row */
-                bool wild = false;
-                if (edge && tb > 1) {
-#pragma unroll
-                    for (int r = 0; r < NR; r++)
-#pragma unroll
-                        for (int i = 0; i < NW; i++) wild |= pg_wild<CT>(b.v[r][i]);
-                    wild = __any(wild);
-                }
-                uint4 pf[NP];                    /* 16-bit caches: the weights' pieces */
-                if constexpr (!F32) {
-                    uint32_t wd[4][NP];
-#pragma unroll
-                    for (int r = 0; r < 4; r++) pg_pieces2<CT, NP>(p[2 * r], p[2 * r + 1], wd[r]);
-#pragma unroll
-                    for (int n = 0; n < NP; n++) pf[n] = make_uint4(wd[0][n], wd[1][n], wd[2][n], wd[3][n]);
-                }
-                /* x plus element j's sum over the keys of the step that `mask` leaves */
-                auto weigh = [&](int j, f32x4_t x, const uint32_t (&mask)[4]) __attribute__((always_inline)) {
-                    if constexpr (F32) {
-#pragma unroll
-                        for (int r = 0; r < 4; r++)
-                            x = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(b.v[r][j] & mask[r]), p[r], x, 0, 0, 0);
-                    } else {
-                        uint32_t vw[4];          /* element j of the eight keys */
-#pragma unroll
-                        for (int r = 0; r < 4; r++)
-                            vw[r] = mask[r] & __builtin_amdgcn_perm(b.v[2 * r + 1][j >> 1], b.v[2 * r][j >> 1],
-                                                                    j & 1 ? 0x07060302u : 0x05040100u);
-                        const uint4 vf = make_uint4(vw[0], vw[1], vw[2], vw[3]);
-#pragma unroll
-                        for (int n = NP - 1; n >= 0; n--) x = pg_mfma16<CT>(vf, pf[n], x);
+                    for (int i = 0; i < 4; i++) {
+                        const int j = jb + 16 * t + 4 * g + i;
+                        st[t][i] = j <= pos && j >= pos_lo ? st[t][i] : -INFINITY;
                     }
-                    return x;
-                };
-                if (!wild) {
-                    const uint32_t all[4] = {~0u, ~0u, ~0u, ~0u};
+            float mn = m;
 #pragma unroll
-                    for (int j = 0; j < DPL; j++) o[j] = weigh(j, o[j], all);
-                } else {                         /* each token's rows from the values that it sees */
-#pragma nounroll
-                    for (int z = 0; z < tb; z++) {
-                        const int ph = first + z, pl = a.b.window > 0 ? ph - a.b.window + 1 : 0;
-                        auto seen = [&](int i) { return jb + i <= ph && jb + i >= pl; };
-                        uint32_t mask[4];
+            for (int t = 0; t < KT / 16; t++)
 #pragma unroll
-                        for (int r = 0; r < 4; r++) {
-                            if constexpr (F32) {
-                                mask[r] = seen(4 * g + r) ? ~0u : 0u;
-                            } else {
-                                const int i = 16 * (r >> 1) + 4 * g + 2 * (r & 1);
-                                mask[r] = (seen(i) ? 0xFFFFu : 0u) | (seen(i + 1) ? 0xFFFF0000u : 0u);
-                            }
-                        }
+                for (int i = 0; i < 4; i++) mn = fmaxf(mn, st[t][i]);
+            mn = fmaxf(mn, __shfl_xor(mn, 16));
+            mn = fmaxf(mn, __shfl_xor(mn, 32));
+            if (__any(mn > m)) {
+                const float Mn = mn == -INFINITY ? 0.0f : cs * mn;
+                const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - Mn);
+                m = mn;
+                M = Mn;
+                l *= f;
 #pragma unroll
-                        for (int j = 0; j < DPL; j++) {
-                            const f32x4_t x = weigh(j, o[j], mask);
-                            if (tok == z) o[j] = x;
-                        }
-                    }
-                }
-                __builtin_amdgcn_sched_barrier(0);
-                load_v(n + 1, id);
-                id = page_of(n + 2);
-                __builtin_amdgcn_sched_barrier(0);
+                for (int j = 0; j < DPL; j++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) o[j][i] *= f;
             }
-            l += __shfl_xor(l, 16);
-            l += __shfl_xor(l, 32);
+            float p[NR];
+#pragma unroll
+            for (int r = 0; r < NR; r++) {
+                p[r] = __builtin_amdgcn_exp2f(fmaf(st[r >> 2][r & 3], cs, P::LIFT - M));
+                l += p[r];
+            }
+            /* values that are no numbers in a step of which some row does not see some key: a
+               weight of zero would not keep them out, so the tokens are taken one by one */
+            bool wild = false;
+            if (edge && tb > 1) {
+                uint32_t any = 0;
+#pragma unroll
+                for (int r = 0; r < NR; r++)
+#pragma unroll
+                    for (int i = 0; i < NW; i++) any |= pg_wild<CT>(b.v[r][i]);
+                wild = __any(any != 0);
+            }
+            uint4 pf[NP];                    /* 16-bit caches: the weights' pieces */
+            if constexpr (!F32) {
+                uint32_t wd[4][NP];
+#pragma unroll
+                for (int r = 0; r < 4; r++) pg_pieces2<CT, NP>(p[2 * r], p[2 * r + 1], wd[r]);
+#pragma unroll
+                for (int n = 0; n < NP; n++) pf[n] = make_uint4(wd[0][n], wd[1][n], wd[2][n], wd[3][n]);
+            }
+            /* x plus element j's sum over the keys of the step that `mask` leaves */
+            auto weigh = [&](int j, f32x4_t x, const uint32_t (&mask)[4]) __attribute__((always_inline)) {
+                if constexpr (F32) {
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+                        x = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(b.v[r][j] & mask[r]), p[r], x, 0, 0, 0);
+                } else {
+                    uint32_t vw[4];          /* element j of the eight keys */
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+                        vw[r] = mask[r] & __builtin_amdgcn_perm(b.v[2 * r + 1][j >> 1], b.v[2 * r][j >> 1],
+                                                                j & 1 ? 0x07060302u : 0x05040100u);
+                    const uint4 vf = make_uint4(vw[0], vw[1], vw[2], vw[3]);
+#pragma unroll
+                    for (int n = NP - 1; n >= 0; n--) x = pg_mfma16<CT>(vf, pf[n], x);
+                }
+                return x;
+            };
+            if (!wild) {
+                const uint32_t all[4] = {~0u, ~0u, ~0u, ~0u};
+#pragma unroll
+                for (int j = 0; j < DPL; j++) o[j] = weigh(j, o[j], all);
+            } else {                         /* a lane's rows are one token's: taken in its turn */
+#pragma nounroll
+                for (int z = 0; z < tb; z++) {
+                    const int ph = first + z, pl = a.b.window > 0 ? ph - a.b.window + 1 : 0;
+                    auto seen = [&](int i) { return jb + i <= ph && jb + i >= pl; };
+                    uint32_t mask[4];
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        if constexpr (F32) {
+                            mask[r] = seen(4 * g + r) ? ~0u : 0u;
+                        } else {
+                            const int i = 16 * (r >> 1) + 4 * g + 2 * (r & 1);
+                            mask[r] = (seen(i) ? 0xFFFFu : 0u) | (seen(i + 1) ? 0xFFFF0000u : 0u);
+                        }
+                    }
+#pragma unroll
+                    for (int j = 0; j < DPL; j++) {
+                        const f32x4_t x = weigh(j, o[j], mask);
+#pragma unroll
+                        for (int i = 0; i < 4; i++) o[j][i] = tok == z ? x[i] : o[j][i];
+                    }
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            load_v(ro);
+            __builtin_amdgcn_sched_barrier(0);
         }
-        /* ---- the four wavefronts' results in one: row r of the tile, element d */
-        if (g == 0) {
-            m_s[w][c] = m == -INFINITY ? -INFINITY : M;
-            l_s[w][c] = l;
+        l += __shfl_xor(l, 16);
+        l += __shfl_xor(l, 32);
+        /* ---- the four wavefronts' results in one: row r of the tile, element d. */
+        int te = tid;
+        asm volatile("" : "+v"(te));
+        const int ce = te & 15, ge = te >> 4 & 3;
+        if (ge == 0) {
+            m_s[w][ce] = m == -INFINITY ? -INFINITY : M;
+            l_s[w][ce] = l;
         }
         __syncthreads();
         {
-            float top = fmaxf(fmaxf(m_s[0][c], m_s[1][c]), fmaxf(m_s[2][c], m_s[3][c]));
+            float top = fmaxf(fmaxf(m_s[0][ce], m_s[1][ce]), fmaxf(m_s[2][ce], m_s[3][ce]));
             const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - top);
 #pragma unroll
             for (int i = 0; i < 4; i++)
 #pragma unroll
-                for (int j = 0; j < DPL; j++) o_s[w][c][DPL * (4 * g + i) + j] = o[j][i] * f;
+                for (int j = 0; j < DPL; j++) o_s[w][ce][DPL * (4 * ge + i) + j] = o[j][i] * f;
         }
         __syncthreads();
+        const pg_args *late = pg_late_args();
         const int rows = tb * a.hpp;
         const bool whole = it.cnt == it.all;
         const int wf = pg_owner(it.first, sh.U, W);
@@ -391,23 +414,34 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_paged_few(const pg_a
         auto finish = [&](int r, int d, float4 v, float top, float L) __attribute__((always_inline)) {
             const int rt = r / a.hpp, rh = it.part * a.hpp + r - rt * a.hpp;
             if (rh >= a.G) return;
-            const int rp = it.q.p0 + t0 + rt, h = it.kv * a.G + rh;
-            const size_t row = (size_t)(it.q.lo + t0 + rt);
+            const int rp = sq.p0 + t0 + rt, h = it.kv * a.G + rh;
+            const size_t row = (size_t)(sq.lo + t0 + rt);
             const float nan = __int_as_float(0x7fc00000);
             float4 y = make_float4(v.x / L, v.y / L, v.z / L, v.w / L);
             /* the lift taken back ahead of the logarithm, exactly */
             float e = (top + __builtin_amdgcn_logf(ldexpf(L, -(int)P::LIFT))) * 0.69314718055994531f;
-            if (it.q.bad) {
+            if (sq.bad) {
                 y = make_float4(nan, nan, nan, nan);
                 e = nan;
             } else if (rp < 0) {
                 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                 e = -INFINITY;
             }
-            pg_put4<AT>(a.out, row * a.ldo + (size_t)h * HD + d, y);
-            if (a.lse && d == 0) a.lse[row * a.H + h] = e;
+            pg_put4<AT>(late->out, row * late->ldo + (size_t)h * HD + d, y);
+            if (late->lse && d == 0) late->lse[row * late->H + h] = e;
         };
-        for (int i = tid; i < rows * (HD / 4); i += 256) {
+        auto put = [&](size_t slot, int r, int d, float4 v, float top, float L) __attribute__((always_inline)) {
+            float *pa = late->pacc + (slot + r) * HD + d;
+            st_agent(pa + 0, v.x);
+            st_agent(pa + 1, v.y);
+            st_agent(pa + 2, v.z);
+            st_agent(pa + 3, v.w);
+            if (d == 0) {
+                st_agent((float *)(late->pml + slot + r), top);
+                st_agent((float *)(late->pml + slot + r) + 1, L);
+            }
+        };
+        for (int i = te; i < rows * (HD / 4); i += 256) {
             const int r = i / (HD / 4), d = i % (HD / 4) * 4;
             float4 v = *(const float4 *)&o_s[0][r][d];
             const float top = fmaxf(fmaxf(m_s[0][r], m_s[1][r]), fmaxf(m_s[2][r], m_s[3][r]));
@@ -423,56 +457,78 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_paged_few(const pg_a
             if (whole) {
                 finish(r, d, v, top, L);
             } else {
-                float *pa = a.pacc + (slot + r) * HD + d;
-                st_agent(pa + 0, v.x);
-                st_agent(pa + 1, v.y);
-                st_agent(pa + 2, v.z);
-                st_agent(pa + 3, v.w);
-                if (d == 0) {
-                    st_agent((float *)(a.pml + slot + r), top);
-                    st_agent((float *)(a.pml + slot + r) + 1, L);
-                }
+                put(slot, r, d, v, top, L);
             }
         }
         if (!whole) {
+            /* The pieces of workgroups wf .. wl. Up to MG of them: the last to arrive merges them.
+               More: the last of each MG merges those into the first one's place, and the last of
+               these merges theirs, so that each round of loads flies at once. A workgroup is the
+               first of an item's pieces, or of a later group of an item's, with a counter for each. */
+            constexpr int MG = 16;
             const int wl = pg_owner(it.first + it.all - 1, sh.U, W);
-            if (last_arriver(&a.ctr[wf], wl - wf, &flag)) {
-                for (int i = tid; i < rows * (HD / 4); i += 256) {
-                    const int r = i / (HD / 4), d = i % (HD / 4) * 4;
-                    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    float top = -INFINITY, L = 0.0f;
-                    for (int x0 = wf; x0 <= wl; x0 += 8) {
-                        f32x2_t ml[8];
-                        float4 y[8];
+            const int gx = wf + (me - wf) / MG * MG, groups = (wl - wf) / MG + 1;
+            auto place = [&](int x) { return ((size_t)2 * x + (x == wf)) * PG_FEW_ROWS; };
+            /* pieces x0, x0 + step, ... (n of them, at most 2 MG) of row r, element d */
+            auto merge = [&](int x0, int n, int step, int r, int d, float4 &v, float &top, float &L)
+                             __attribute__((always_inline)) {
+                v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                top = -INFINITY;
+                L = 0.0f;
+                for (int k0 = 0; k0 < n; k0 += MG) {
+                    f32x2_t ml[MG];
+                    float4 y[MG];
 #pragma unroll
-                        for (int k = 0; k < 8; k++) {
-                            const int x = min(x0 + k, wl);
-                            const size_t sl = ((size_t)2 * x + (x == wf)) * PG_FEW_ROWS + r;
-                            const unsigned long long b = ld_agent((const unsigned long long *)(a.pml + sl));
-                            ml[k] = f32x2_t{__uint_as_float((uint32_t)b), __uint_as_float((uint32_t)(b >> 32))};
-                            const v4i_t z = ld_agent16(a.pacc, (uint32_t)((sl * HD + d) * 4));
-                            y[k] = make_float4(__int_as_float(z.x), __int_as_float(z.y),
-                                               __int_as_float(z.z), __int_as_float(z.w));
-                        }
-                        float t2 = top;
+                    for (int k = 0; k < MG; k++) {
+                        const size_t sl = place(x0 + min(k0 + k, n - 1) * step) + r;
+                        const unsigned long long b = ld_agent((const unsigned long long *)(late->pml + sl));
+                        ml[k] = f32x2_t{__uint_as_float((uint32_t)b), __uint_as_float((uint32_t)(b >> 32))};
+                        const v4i_t z = ld_agent16(late->pacc, (uint32_t)((sl * HD + d) * 4));
+                        y[k] = make_float4(__int_as_float(z.x), __int_as_float(z.y),
+                                           __int_as_float(z.z), __int_as_float(z.w));
+                    }
+                    float t2 = top;
 #pragma unroll
-                        for (int k = 0; k < 8; k++) t2 = fmaxf(t2, ml[k].x);
-                        const float f = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - t2);
-                        top = t2;
-                        L *= f;
-                        v = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
+                    for (int k = 0; k < MG; k++) t2 = fmaxf(t2, ml[k].x);
+                    const float f = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - t2);
+                    top = t2;
+                    L *= f;
+                    v = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
 #pragma unroll
-                        for (int k = 0; k < 8; k++) {
-                            if (x0 + k > wl) break;
-                            const float e = ml[k].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml[k].x - top);
-                            L = fmaf(e, ml[k].y, L);
-                            v = make_float4(fmaf(e, y[k].x, v.x), fmaf(e, y[k].y, v.y),
-                                            fmaf(e, y[k].z, v.z), fmaf(e, y[k].w, v.w));
+                    for (int k = 0; k < MG; k++) {
+                        if (k0 + k < n) {
+                        const float e = ml[k].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml[k].x - top);
+                        L = fmaf(e, ml[k].y, L);
+                        v = make_float4(fmaf(e, y[k].x, v.x), fmaf(e, y[k].y, v.y),
+                                        fmaf(e, y[k].z, v.z), fmaf(e, y[k].w, v.w));
                         }
                     }
-                    finish(r, d, v, top, L);
+                }
+            };
+            bool mine = true;
+            if (groups > 1) {
+                const int n = min(MG, wl - gx + 1);
+                mine = last_arriver(&late->ctr[2 * gx + (gx == wf)], n - 1, &flag);
+                if (mine) {
+                    for (int i0 = 0; i0 < rows * (HD / 4); i0 += 256) {
+                        const int i = i0 + te, ic = min(i, rows * (HD / 4) - 1);
+                        const int r = ic / (HD / 4), d = ic % (HD / 4) * 4;
+                        float4 v;
+                        float top, L;
+                        merge(gx, n, 1, r, d, v, top, L);
+                        __syncthreads();         /* every thread of the row has read its (M, l) */
+                        if (i < rows * (HD / 4)) put(place(gx), r, d, v, top, L);
+                    }
                 }
             }
+            if (mine && last_arriver(&late->ctr[2 * W + wf], groups > 1 ? groups - 1 : wl - wf, &flag))
+                for (int i = te; i < rows * (HD / 4); i += 256) {
+                    const int r = i / (HD / 4), d = i % (HD / 4) * 4;
+                    float4 v;
+                    float top, L;
+                    merge(wf, groups > 1 ? groups : wl - wf + 1, groups > 1 ? MG : 1, r, d, v, top, L);
+                    finish(r, d, v, top, L);
+                }
         }
         __syncthreads();                         /* LDS is free for the next item */
     }

@@ -17,7 +17,8 @@ static int below(int n) {
 }
 
 /* units of tile i, by the keys that its rows see */
-static int count_units(const pg_seq &s, int tl, int window, int i, int *lo_unit) {
+static int count_units(const pg_batch &b, const pg_seq &s, int i, int *lo_unit) {
+    const int tl = b.tl, window = b.window, unit = 1 << b.ul;
     int lo = -1, hi = -1;
     for (int t = i << tl; t < s.n && t < (i + 1) << tl; t++) {
         const int pos = s.p0 + t;
@@ -27,14 +28,14 @@ static int count_units(const pg_seq &s, int tl, int window, int i, int *lo_unit)
         if (pos > hi) hi = pos;
     }
     if (hi < 0) { *lo_unit = 0; return 1; }
-    *lo_unit = lo / PG_UNIT;
-    return hi / PG_UNIT - lo / PG_UNIT + 1;
+    *lo_unit = lo / unit;
+    return hi / unit - lo / unit + 1;
 }
 
 static int check(const std::vector<int> &off, const std::vector<int> &len, int T, int KV, int parts, int tl,
-                 int window, int plog, int max_pages, int grid) {
+                 int ul, int window, int plog, int max_pages, int grid) {
     const int S = (int)len.size();
-    const pg_batch b = {off.data(), len.data(), S, T, KV, max_pages, plog, window, parts, tl};
+    const pg_batch b = {off.data(), len.data(), S, T, KV, max_pages, plog, window, parts, tl, ul};
     int64_t U = 0;
     std::vector<int64_t> before(S);
     for (int s = 0; s < S; s++) {
@@ -42,33 +43,33 @@ static int check(const std::vector<int> &off, const std::vector<int> &len, int T
         if (q.lo < 0 || q.n < 0 || q.lo + q.n > T || q.len < 0) { printf("bad rows of %d\n", s); return 1; }
         int64_t sum = 0;
         for (int i = 0; i <= pg_tiles(q, tl); i++) {
-            if (q.n && pg_units_before(q, tl, window, i) != sum) {
+            if (q.n && pg_units_before(b, q, i) != sum) {
                 printf("units before tile %d of n=%d len=%d tl=%d window=%d: %lld, counted %lld\n", i, q.n,
-                       q.len, tl, window, (long long)pg_units_before(q, tl, window, i), (long long)sum);
+                       q.len, tl, window, (long long)pg_units_before(b, q, i), (long long)sum);
                 return 1;
             }
             if (i == pg_tiles(q, tl)) break;
             int lo;
-            const int c = count_units(q, tl, window, i, &lo);
-            if (q.p0 + q.n > 0 && q.p0 + ((i + 1) << tl) > 0 && q.len > 0 && lo != pg_unit_lo(q, tl, window, i)) {
+            const int c = count_units(b, q, i, &lo);
+            if (q.p0 + q.n > 0 && q.p0 + ((i + 1) << tl) > 0 && q.len > 0 && lo != pg_unit_lo(b, q, i)) {
                 printf("first unit of tile %d\n", i);
                 return 1;
             }
             sum += c;
         }
+        if (pg_seq_units(b, q) != sum * KV * parts) { printf("units of %d\n", s); return 1; }
         before[s] = U;
         U += sum * KV * parts;
     }
     /* the walks */
     std::map<std::tuple<int, int, int, int>, std::vector<int>> met;   /* item -> owner of each unit */
-    std::map<std::tuple<int, int, int, int>, int64_t> firsts;
+    std::map<std::tuple<int, int, int, int>, uint32_t> firsts;
     int64_t next = 0;
     for (int w = 0; w < grid && U; w++) {
         pg_share r;
-        r.U = U;
         int block = 0;                           /* the block that takes share w */
         for (; block < grid; block++) {
-            pg_deal(r, block, grid);
+            r = pg_deal((uint32_t)U, block, grid);
             if (r.w == w) break;
         }
         if (block == grid) { printf("no block for share %d of %d\n", w, grid); return 1; }
@@ -79,17 +80,23 @@ static int check(const std::vector<int> &off, const std::vector<int> &len, int T
         if (r.u0 != next || r.u1 <= r.u0) { printf("share %d: %lld..%lld after %lld\n", w, (long long)r.u0, (long long)r.u1, (long long)next); return 1; }
         next = r.u1;
         int s = S - 1;
-        while (before[s] > r.u0 || (s > 0 && before[s] == before[s - 1] && before[s] > r.u0)) s--;
+        while (before[s] > r.u0) s--;
         int64_t rem = r.u0 - before[s];
-        for (int64_t u = r.u0; u < r.u1;) {
-            const pg_item it = pg_next_item(b, u, r.u1, s, rem);
+        for (uint32_t u = r.u0; u < r.u1;) {
+            pg_seq q = pg_get_seq(b.q_off, b.len, s, T, max_pages, plog);
+            while (rem >= pg_seq_units(b, q)) {
+                q = pg_get_seq(b.q_off, b.len, ++s, T, max_pages, plog);
+                rem = 0;
+            }
+            const pg_item it = pg_find_item(b, q, u, r.u1, (uint32_t)rem);
+            rem += it.cnt;
             if (it.cnt <= 0 || it.off < 0 || it.off + it.cnt > it.all || u + it.cnt > r.u1) { printf("bad item\n"); return 1; }
-            auto key = std::make_tuple(it.s, it.kv, it.part, it.tile);
+            auto key = std::make_tuple(s, it.kv, it.part, it.tile);
             if (!met.count(key)) firsts[key] = it.first;
             if (firsts[key] != it.first || (int)met[key].size() != it.off) { printf("pieces out of order\n"); return 1; }
             for (int i = 0; i < it.cnt; i++) met[key].push_back(w);
             if ((int)met[key].size() == it.all) {
-                const int wf = pg_owner(it.first, U, r.W), wl = pg_owner(it.first + it.all - 1, U, r.W);
+                const int wf = pg_owner(it.first, (uint32_t)U, r.W), wl = pg_owner(it.first + it.all - 1, (uint32_t)U, r.W);
                 int pieces = 1;
                 for (int i = 1; i < it.all; i++) pieces += met[key][i] != met[key][i - 1];
                 if (wf != met[key][0] || wl != w || wl - wf + 1 != pieces) { printf("owners %d..%d, met %d..%d\n", wf, wl, met[key][0], w); return 1; }
@@ -104,7 +111,7 @@ static int check(const std::vector<int> &off, const std::vector<int> &len, int T
             for (int p = 0; p < parts; p++)
                 for (int i = 0; i < pg_tiles(q, tl); i++) {
                     int lo;
-                    if ((int)met[std::make_tuple(s, kv, p, i)].size() != count_units(q, tl, window, i, &lo)) {
+                    if ((int)met[std::make_tuple(s, kv, p, i)].size() != count_units(b, q, i, &lo)) {
                         printf("item (%d, %d, %d, %d) not whole\n", s, kv, p, i);
                         return 1;
                     }
@@ -136,14 +143,20 @@ int main() {
             else off[s + 1] = below(2) ? -5 : T + 7;
         }
         const int window = below(2) ? 0 : 1 + below(below(2) ? 20 : 500);
-        if (check(off, len, T, 1 + below(4), 1 + below(2), tl, window, plog, max_pages, grids[below(7)])) {
+        if (check(off, len, T, 1 + below(4), 1 + below(2), tl, tl + below(9 - tl), window, plog, max_pages, grids[below(7)])) {
             printf("case %d\n", c);
             return 1;
         }
     }
-    /* the largest: no sum leaves 64 bits, no position 32 */
-    const pg_seq big = {0, 1 << 20, PG_MAX_LEN, PG_MAX_LEN - (1 << 20), false, false};
-    if (pg_units_before(big, 0, 0, 1 << 20) <= (int64_t)(PG_MAX_LEN - (1 << 20)) / PG_UNIT * (1 << 20)) return 1;
+    /* the largest positions: a sum that leaves 32 bits, differences that do not */
+    const pg_seq big = {0, 1 << 10, PG_MAX_LEN, PG_MAX_LEN - (1 << 10), false, false};
+    const pg_batch b = {nullptr, nullptr, 1, 1 << 10, 1, 0, 0, 0, 1, 0, 12};
+    uint32_t sum = 0;
+    for (int i = 0; i < 1 << 10; i++) {
+        int lo;
+        if (pg_units_before(b, big, i) != sum) return 1;
+        sum += count_units(b, big, i, &lo);
+    }
     printf("ok\n");
     return 0;
 }
