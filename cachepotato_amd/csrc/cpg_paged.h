@@ -8,6 +8,8 @@
 
 #define PG_FEW_ROWS 16      /* query rows of a tile of k_paged_few: one MFMA tile */
 #define PG_FEW_WGS 512      /* workgroups of k_paged_few at most: two per CU */
+#define PG_MANY_ROWS 128    /* query rows of a tile of k_paged_many: 32 to a wavefront */
+#define PG_MANY_WGS 512     /* workgroups of k_paged_many at most: two per CU */
 
 /* one call of cpg_paged_attn, as the kernels get it. Row offsets in the pool are taken in units of
    2^ush bytes, the largest power of two that divides both strides, so that they fit 32 bits. */
@@ -52,6 +54,7 @@ struct cpg_paged_ws {
 };
 
 int pg_launch_few(const pg_args &a, int type, int cache, int HD, int grid);
+int pg_launch_many(const pg_args &a, int type, int cache, int HD, int grid);
 
 /* ---------------------------------------------------------------- element types */
 
@@ -83,6 +86,57 @@ template <int TYPE> __device__ static inline void pg_put4(void *p, size_t i, flo
         *(float4 *)((float *)p + i) = v;
     else
         *(uint2 *)((uint16_t *)p + i) = make_uint2(pg_pack2<TYPE>(v.x, v.y), pg_pack2<TYPE>(v.z, v.w));
+}
+
+/* (x, y) as NP pieces of CT, a pair to a word */
+template <int CT, int NP>
+__device__ static inline void pg_pieces2(float x, float y, uint32_t (&w)[NP]) {
+    if constexpr (NP == 1) {
+        w[0] = pg_pack2<CT>(x, y);
+    } else if constexpr (NP == 2) {
+        const f16pair2 p = split_f16x2(x, y);
+        w[0] = p.hi;
+        w[1] = p.lo;
+    } else {                                     /* leading bits, leading bits of the rest, the rest */
+        const uint32_t xa = __float_as_uint(x), ya = __float_as_uint(y);
+        const float xr = x - __uint_as_float(xa & 0xFFFF0000u), yr = y - __uint_as_float(ya & 0xFFFF0000u);
+        const uint32_t xb = __float_as_uint(xr), yb = __float_as_uint(yr);
+        const float xs = xr - __uint_as_float(xb & 0xFFFF0000u), ys = yr - __uint_as_float(yb & 0xFFFF0000u);
+        w[0] = __builtin_amdgcn_perm(ya, xa, 0x07060302u);
+        w[1] = __builtin_amdgcn_perm(yb, xb, 0x07060302u);
+        w[2] = __builtin_amdgcn_perm(__float_as_uint(ys), __float_as_uint(xs), 0x07060302u);
+    }
+}
+
+/* the top bit of a word (of both its halves, for 16-bit types) set where the exponent is all ones,
+   an infinity's or a NaN's: one step more carries into it. Words, not truth values, which would
+   fill the scalar registers. */
+template <int CT> __device__ static inline uint32_t pg_wild(uint32_t w) {
+    constexpr uint32_t E = CT == CPG_T_F32 ? 0x7F800000u : CT == CPG_T_F16 ? 0x7C007C00u : 0x7F807F80u;
+    constexpr uint32_t ONE = CT == CPG_T_F32 ? 0x00800000u : CT == CPG_T_F16 ? 0x04000400u : 0x00800080u;
+    return ((w & E) + ONE) & (CT == CPG_T_F32 ? 0x80000000u : 0x80008000u);
+}
+/* An address computed as a number, for loads from global memory: as a generic pointer its loads
+   would count as LDS operations too, and every LDS read would wait for all of them. */
+template <typename T> __device__ static inline T pg_load(uint64_t p) {
+    return *(const __attribute__((address_space(1))) T *)p;
+}
+
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+
+/* the address of a row at offset r of the pool (of keys or of values) */
+__device__ static inline uint64_t pg_row_ptr(const uint8_t *base, uint32_t r, int ush, const uint8_t *blank, bool key) {
+    const uint64_t p = (uint64_t)base + ((uint64_t)r << ush);
+    const uint64_t no = (uint64_t)blank + (key && r == PG_BAD_ROW ? 1024 : 0);
+    return r >= PG_BAD_ROW ? no : p;
+}
+
+/* 16 bytes stored for another workgroup of this launch (st_agent's form, four words at once) */
+__device__ static inline void pg_st_agent16(void *base, uint32_t off, float4 v) {
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(base, 0, 0x7fffffff, 0x00020000);
+    __builtin_amdgcn_raw_buffer_store_b128(
+        v4i_t{__float_as_int(v.x), __float_as_int(v.y), __float_as_int(v.z), __float_as_int(v.w)}, r, off, 0, 16);
 }
 
 /* ---------------------------------------------------------------- shares */

@@ -251,7 +251,7 @@ extern "C" cpg_paged_ws *cpg_paged_ws_create(int H, int KV, int HD) {
     ws->H = H;
     ws->KV = KV;
     ws->HD = HD;
-    ws->rows = (size_t)2 * PG_FEW_WGS * PG_FEW_ROWS;
+    ws->rows = (size_t)2 * PG_MANY_WGS * PG_MANY_ROWS;     /* k_paged_few needs an eighth */
     const size_t sz[5] = {ws->rows * HD * 4, ws->rows * 8, (size_t)3 * PG_FEW_WGS * 4, 4, 2048};
     size_t total = 0;
     for (int i = 0; i < 5; i++) total += cpg_round256(sz[i]);
@@ -371,13 +371,15 @@ extern "C" int cpg_paged_attn(const cpg_paged_cache *C, const cpg_paged_batch *B
     a.scale2 = (scale > 0.0f ? scale : 1.0f / sqrtf((float)C->HD)) * 1.4426950408889634f;
     a.blank = ws->blank;
     a.pacc = ws->pacc; a.pml = ws->pml; a.ctr = ws->ctr; a.stat = ws->stat;
-    const int rows = PG_FEW_ROWS;
+    const bool few = (int64_t)B->max_new * a.G <= PG_FEW_ROWS;
+    const int rows = few ? PG_FEW_ROWS : PG_MANY_ROWS;
     a.hpp = a.G < rows ? a.G : rows;
-    /* a unit is one step of a workgroup's four wavefronts: 64 keys of an f32 cache, 128 of a 16-bit
-       one (more where the units of the largest batch there can be would not fit 31 bits) */
+    /* a unit is 128 keys: one step of the four wavefronts of k_paged_few for a 16-bit cache (half
+       as many for an f32 one), two or four steps of k_paged_many; more where the units of the
+       largest batch there can be would not fit 31 bits */
     a.b = pg_batch{B->q_off, B->len, B->S, B->T, C->KV, B->max_pages, log2_of(C->page),
                    window < PG_MAX_LEN ? window : 0, (a.G + a.hpp - 1) / a.hpp, 0,
-                   C->type == CPG_T_F32 ? 6 : 7};
+                   few && C->type == CPG_T_F32 ? 6 : 7};
     while ((2 << a.b.tl) * a.hpp <= rows) a.b.tl++;
     /* no more workgroups than units there can be: tiles of the rows, and keys of a full page row */
     const double tiles = (double)(B->T >> a.b.tl) + (B->S < B->T ? B->S : B->T);
@@ -390,6 +392,8 @@ extern "C" int cpg_paged_attn(const cpg_paged_cache *C, const cpg_paged_batch *B
         cpg_set_error("cpg_paged_attn: a batch of %d rows and %d sequences of %d heads is too large", B->T, B->S, H);
         return -1;
     }
-    const int grid = units < PG_FEW_WGS ? (int)units : PG_FEW_WGS;
+    const int most = few ? PG_FEW_WGS : C->HD <= 128 ? PG_MANY_WGS : PG_MANY_WGS / 2;
+    const int grid = units < most ? (int)units : most;
+    if (!few) return pg_launch_many(a, type, C->type, C->HD, grid);
     return pg_launch_few(a, type, C->type, C->HD, grid);
 }

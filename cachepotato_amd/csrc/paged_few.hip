@@ -46,26 +46,6 @@ __device__ static inline f32x4_t pg_mfma16(uint4 a, uint4 b, f32x4_t c) {
                                                        __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
 }
 
-/* (x, y) as NP pieces of CT, a pair to a word */
-template <int CT, int NP>
-__device__ static inline void pg_pieces2(float x, float y, uint32_t (&w)[NP]) {
-    if constexpr (NP == 1) {
-        w[0] = pg_pack2<CT>(x, y);
-    } else if constexpr (NP == 2) {
-        const f16pair2 p = split_f16x2(x, y);
-        w[0] = p.hi;
-        w[1] = p.lo;
-    } else {                                     /* leading bits, leading bits of the rest, the rest */
-        const uint32_t xa = __float_as_uint(x), ya = __float_as_uint(y);
-        const float xr = x - __uint_as_float(xa & 0xFFFF0000u), yr = y - __uint_as_float(ya & 0xFFFF0000u);
-        const uint32_t xb = __float_as_uint(xr), yb = __float_as_uint(yr);
-        const float xs = xr - __uint_as_float(xb & 0xFFFF0000u), ys = yr - __uint_as_float(yb & 0xFFFF0000u);
-        w[0] = __builtin_amdgcn_perm(ya, xa, 0x07060302u);
-        w[1] = __builtin_amdgcn_perm(yb, xb, 0x07060302u);
-        w[2] = __builtin_amdgcn_perm(__float_as_uint(ys), __float_as_uint(xs), 0x07060302u);
-    }
-}
-
 /* the registers of one step: KT key rows and value rows */
 template <int CT, int HD> struct pg_buf {
     static constexpr bool F32 = CT == CPG_T_F32;
@@ -76,15 +56,6 @@ template <int CT, int HD> struct pg_buf {
     uint4 k[NK];
     uint32_t v[NR][NW];
 };
-
-/* An address computed as a number, for loads from global memory: as a generic pointer its loads
-   would count as LDS operations too, and every LDS read would wait for all of them. */
-template <typename T> __device__ static inline T pg_load(uint64_t p) {
-    return *(const __attribute__((address_space(1))) T *)p;
-}
-
-typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 
 template <int NW> __device__ static inline void pg_load_words(uint64_t p, uint32_t (&w)[NW]) {
     /* the lane's part of a row starts on a multiple of 4 NW bytes of it */
@@ -106,14 +77,6 @@ template <int NW> __device__ static inline void pg_load_words(uint64_t p, uint32
     }
 }
 
-/* the top bit of a word (of both its halves, for 16-bit types) set where the exponent is all ones,
-   an infinity's or a NaN's: one step more carries into it. Words, not truth values, which would
-   fill the scalar registers. */
-template <int CT> __device__ static inline uint32_t pg_wild(uint32_t w) {
-    constexpr uint32_t E = CT == CPG_T_F32 ? 0x7F800000u : CT == CPG_T_F16 ? 0x7C007C00u : 0x7F807F80u;
-    constexpr uint32_t ONE = CT == CPG_T_F32 ? 0x00800000u : CT == CPG_T_F16 ? 0x04000400u : 0x00800080u;
-    return ((w & E) + ONE) & (CT == CPG_T_F32 ? 0x80000000u : 0x80008000u);
-}
 /* grid W workgroups of 256 threads, each with its share of the units (cpg_paged.h) */
 template <int CT, int AT, int HD>
 __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_paged_few(const pg_args a) {
@@ -188,9 +151,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_paged_few(const pg_a
             return out ? PG_NO_ROW : miss ? PG_BAD_ROW : r;
         };
         auto row_ptr = [&](const uint8_t *base, uint32_t r, bool key) __attribute__((always_inline)) {
-            const uint64_t p = (uint64_t)base + ((uint64_t)r << a.ush);
-            const uint64_t no = (uint64_t)a.blank + (key && r == PG_BAD_ROW ? 1024 : 0);
-            return r >= PG_BAD_ROW ? no : p;
+            return pg_row_ptr(base, r, a.ush, a.blank, key);
         };
         buf b;
         auto load_k = [&](uint32_t ro) __attribute__((always_inline)) {
