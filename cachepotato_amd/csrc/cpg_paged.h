@@ -116,6 +116,11 @@ template <int CT> __device__ static inline uint32_t pg_wild(uint32_t w) {
     constexpr uint32_t ONE = CT == CPG_T_F32 ? 0x00800000u : CT == CPG_T_F16 ? 0x04000400u : 0x00800080u;
     return ((w & E) + ONE) & (CT == CPG_T_F32 ? 0x80000000u : 0x80008000u);
 }
+/* a word with its infinities and NaNs replaced by zero */
+template <int CT> __device__ static inline uint32_t pg_tame(uint32_t w) {
+    const uint32_t t = pg_wild<CT>(w);
+    return w & ~(t | (t - (t >> (CT == CPG_T_F32 ? 31 : 15))));
+}
 /* An address computed as a number, for loads from global memory: as a generic pointer its loads
    would count as LDS operations too, and every LDS read would wait for all of them. */
 template <typename T> __device__ static inline T pg_load(uint64_t p) {

@@ -46,6 +46,7 @@ template <int CT, int AT, int HD> struct pg_many_t {
     /* 16-bit: copies of 1 KiB per wavefront and step, and rows in each. f32: chunks per thread */
     static constexpr int CHUNKS = KT * (HD / 8);
     static constexpr int E = F32 ? (CHUNKS + 255) / 256 : PLANE / 4096, RPE = 64 / CPR;
+    static constexpr size_t SLOT = (size_t)PG_MANY_ROWS * HD * 4;  /* bytes of a piece */
     static constexpr float LIFT = OT == CPG_T_F16 ? 4.0f : 0.0f;
     __host__ __device__ static constexpr int kswz(int r) { return CPR == 8 ? (r >> 1) & 7 : r & 15; }
     __host__ __device__ static constexpr int vswz(int r) { return CPR == 8 ? ((r >> 1) & 3) << 1 : (r & 7) << 1; }
@@ -144,27 +145,33 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_paged_many(const pg_
         auto row_e = [&](int e) __attribute__((always_inline)) {
             return F32 ? min(tid + 256 * e, P::CHUNKS - 1) / (HD / 8) : (w * E + e) * P::RPE + lane / CPR;
         };
-        int id[E];
-        uint32_t ro[E];
-        auto load_ids = [&](int n) __attribute__((always_inline)) {
-#pragma unroll
-            for (int e = 0; e < E; e++) {
-                const int j = j0 + KT * n + row_e(e);
-                id[e] = ids[max(min(max(j, klo), khi - 1), 0) >> a.b.plog];
+        /* the row of the step that lane l % KT finds for all: the page of its key, in another register
+           while that flies, and the row's offset. A key that no row sees stands for one that does
+           (its score is masked; should its value be no number, that is noted below) */
+        auto key_of = [&](int n) { return max(min(max(j0 + KT * n + lane % KT, klo), khi - 1), 0); };
+        auto load_id = [&](int n) { return ids[key_of(n) >> a.b.plog]; };
+        uint32_t ro;
+        bool lost;                               /* a bad page id among the step's */
+        auto make_rows = [&](int n, int id) __attribute__((always_inline)) {
+            const bool miss = (uint32_t)id >= (uint32_t)a.n_pages;
+            ro = (uint32_t)id * a.page_units + (uint32_t)(key_of(n) & pmask) * a.slot_units;
+            lost = __any(miss);
+            if (lost) {
+                ro = miss ? PG_BAD_ROW : ro;
+                if (lane == 0 && khi > 0) *pg_late_args()->stat = 1;     /* no key: no page is needed */
             }
         };
-        /* a key that no row sees reads zeros; a bad page id makes the key NaN, and its scores */
-        auto make_rows = [&](int n) __attribute__((always_inline)) {
-            bool lost = false;
-#pragma unroll
-            for (int e = 0; e < E; e++) {
-                const int j = j0 + KT * n + row_e(e);
-                const bool out = j < klo || j >= khi, miss = (uint32_t)id[e] >= (uint32_t)a.n_pages;
-                lost |= miss && !out;
-                const uint32_t r = (uint32_t)id[e] * a.page_units + (uint32_t)(j & pmask) * a.slot_units;
-                ro[e] = out ? PG_NO_ROW : miss ? PG_BAD_ROW : r;
+        /* the addresses of row i of the step: of its key (a bad page's: NaN, and its scores with it)
+           and of its value */
+        auto rows_at = [&](int i, uint64_t &kp, uint64_t &vp) __attribute__((always_inline)) {
+            const uint32_t r = __shfl(ro, i);
+            const uint64_t off = (uint64_t)r << a.ush;
+            kp = (uint64_t)kb + off;
+            vp = (uint64_t)vb + off;
+            if (lost && r == PG_BAD_ROW) {
+                kp = (uint64_t)a.blank + 1024;
+                vp = (uint64_t)a.blank;
             }
-            if (__any(lost) && lane == 0) *pg_late_args()->stat = 1;
         };
         const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_u8 *)lds;
         auto copy = [&](int buf) __attribute__((always_inline)) {
@@ -173,8 +180,10 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_paged_many(const pg_
                 const int r = row_e(e), pc = lane % CPR;
                 const uint32_t dst = lds0 + buf * P::BUF + (w * E + e) * 1024;
                 const int kc = min(pc ^ P::kswz(r), HD / 8 - 1), vc = min(pc ^ P::vswz(r), HD / 8 - 1);
-                pg_dma16(pg_row_ptr(kb, ro[e], a.ush, a.blank, true) + 16 * kc, dst);
-                pg_dma16(pg_row_ptr(vb, ro[e], a.ush, a.blank, false) + 16 * vc, dst + P::PLANE);
+                uint64_t kp, vp;
+                rows_at(r, kp, vp);
+                pg_dma16(kp + 16 * kc, dst);
+                pg_dma16(vp + 16 * vc, dst + P::PLANE);
             }
         };
         constexpr int EF = F32 ? E : 1;
@@ -183,12 +192,12 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_paged_many(const pg_
 #pragma unroll
             for (int e = 0; e < EF; e++) {
                 const uint64_t d = 32 * (min(tid + 256 * e, P::CHUNKS - 1) % (HD / 8));
-                const uint64_t kp = pg_row_ptr(kb, ro[e], a.ush, a.blank, true) + d;
-                const uint64_t vp = pg_row_ptr(vb, ro[e], a.ush, a.blank, false) + d;
+                uint64_t kp, vp;
+                rows_at(row_e(e), kp, vp);
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
-                    kraw[e][i] = pg_load<u32x4_t>(kp + 16 * i);
-                    vraw[e][i] = pg_load<u32x4_t>(vp + 16 * i);
+                    kraw[e][i] = pg_load<u32x4_t>(kp + d + 16 * i);
+                    vraw[e][i] = pg_load<u32x4_t>(vp + d + 16 * i);
                 }
             }
         };
@@ -216,21 +225,27 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_paged_many(const pg_
         };
         /* whether step n lies across the border of what the tile's rows see */
         auto crosses = [&](int n) { return j0 + KT * n < (a.b.window > 0 ? max(0, last - a.b.window + 1) : 0) || j0 + KT * n + KT - 1 > first; };
-        /* step n's values that are no numbers, where some row does not see some key: noted for the
-           workgroup by the wavefronts that staged them */
+        /* Infinities and NaNs among the values of a step of which some row does not see some key: a weight
+           of zero would not keep them out of that row's sums. They are taken out of LDS by the
+           wavefronts that staged them, and added where they are seen (below). */
         auto note = [&](int n, int buf, int turn) __attribute__((always_inline)) {
-            if (tb <= 1 || !crosses(n)) return;
+            if (!crosses(n)) return;
             uint32_t any = 0;
             if constexpr (F32) {
 #pragma unroll
                 for (int e = 0; e < EF; e++)
 #pragma unroll
-                    for (int i = 0; i < 8; i++) any |= pg_wild<CPG_T_F32>(vraw[e][i >> 2][i & 3]);
+                    for (int i = 0; i < 8; i++) {
+                        any |= pg_wild<CPG_T_F32>(vraw[e][i >> 2][i & 3]);
+                        vraw[e][i >> 2][i & 3] = pg_tame<CPG_T_F32>(vraw[e][i >> 2][i & 3]);
+                    }
             } else {
 #pragma unroll
                 for (int e = 0; e < E; e++) {
-                    const uint4 x = *(const uint4 *)(lds + buf * P::BUF + P::PLANE + (w * E + e) * 1024 + 16 * lane);
+                    uint4 *p = (uint4 *)(lds + buf * P::BUF + P::PLANE + (w * E + e) * 1024 + 16 * lane);
+                    const uint4 x = *p;
                     any |= pg_wild<CT>(x.x) | pg_wild<CT>(x.y) | pg_wild<CT>(x.z) | pg_wild<CT>(x.w);
+                    *p = make_uint4(pg_tame<CT>(x.x), pg_tame<CT>(x.y), pg_tame<CT>(x.z), pg_tame<CT>(x.w));
                 }
             }
             if (__any(any != 0)) wild_s[turn & 3] = 1;
@@ -241,7 +256,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_paged_many(const pg_
         for (int d = 0; d < ND; d++) o[d] = f32x16_t{};
         float M = -INFINITY, l = 0.0f;           /* what the weights refer to, in log2; -inf: nothing yet */
 
-        load_ids(0);
+        int id = load_id(0);
         /* ---- the queries */
         uint4 qf[NQ][NS];
         float cs = a.scale2;
@@ -282,15 +297,15 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_paged_many(const pg_
             }
         }
         /* the first step into buffer 0 */
-        make_rows(0);
+        make_rows(0, id);
         if constexpr (F32) {
             fetch();
-            load_ids(1);
+            id = load_id(1);
             note(0, 0, turn);
             store(0);
         } else {
             copy(0);
-            load_ids(1);
+            id = load_id(1);
             wait_vm_lgkm<0>();
             note(0, 0, turn);
         }
@@ -305,10 +320,10 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_paged_many(const pg_
             const int jb = j0 + KT * n, buf = n & 1;
             const bool more = n + 1 < steps;
             if (more) {
-                make_rows(n + 1);
+                make_rows(n + 1, id);
                 if constexpr (F32) fetch();
                 else copy(buf ^ 1);
-                load_ids(n + 2);
+                id = load_id(n + 2);
             }
             if (active && jb <= wlast && jb + KT > wklo) {
                 const uint8_t *base = lds + buf * P::BUF;
@@ -360,8 +375,9 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_paged_many(const pg_
                         for (int i = 0; i < 16; i++) o[d][i] *= f;
                 }
                 const float off = P::LIFT - (M == -INFINITY ? 0.0f : M);
-                const bool wild = edge && tb > 1 && wild_s[turn & 3] != 0;
-                /* weights of 16 keys, then their share of the sums */
+                const bool wild = crosses(n) && wild_s[turn & 3] != 0;
+                /* the weights, 16 keys to an operand */
+                uint4 pf[2 * NB][NQ];
 #pragma unroll
                 for (int k = 0; k < 2 * NB; k++) {
                     uint32_t wd[4][NQ];
@@ -373,62 +389,80 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_paged_many(const pg_
                         l += y;
                         pg_pieces2<OT, NQ>(x, y, wd[i]);
                     }
-                    uint4 pf[NQ];
 #pragma unroll
-                    for (int p = 0; p < NQ; p++) pf[p] = make_uint4(wd[0][p], wd[1][p], wd[2][p], wd[3][p]);
-                    auto values = [&](int d, uint4 (&vf)[NC]) __attribute__((always_inline)) {
+                    for (int p = 0; p < NQ; p++) pf[k][p] = make_uint4(wd[0][p], wd[1][p], wd[2][p], wd[3][p]);
+                }
+                /* elements 32 d .. of the values of keys 16 k .. */
+                auto values = [&](int k, int d, uint4 (&vf)[NC]) __attribute__((always_inline)) {
 #pragma unroll
-                        for (int p = 0; p < NC; p++) {
-                            const uint8_t *vp = base + p * P::PLANE + 16 * k * RB + (vread ^ (d << 6));
-                            const uint2 lo = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                (__attribute__((address_space(3))) s16x4_t *)(lds_u8 *)vp));
-                            const uint2 hi = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                (__attribute__((address_space(3))) s16x4_t *)(lds_u8 *)(vp + 8 * RB)));
-                            vf[p] = make_uint4(lo.x, lo.y, hi.x, hi.y);
-                        }
-                    };
-                    auto weigh = [&](const uint4 (&vf)[NC], f32x16_t x) __attribute__((always_inline)) {
-                        if constexpr (F32) {
-                            x = pg_mfma32<OT>(vf[1], pf[0], x);
-                            x = pg_mfma32<OT>(vf[0], pf[1], x);
-                            return pg_mfma32<OT>(vf[0], pf[0], x);
-                        } else {
+                    for (int p = 0; p < NC; p++) {
+                        const uint8_t *vp = base + p * P::PLANE + 16 * k * RB + (vread ^ (d << 6));
+                        const uint2 lo = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                            (__attribute__((address_space(3))) s16x4_t *)(lds_u8 *)vp));
+                        const uint2 hi = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                            (__attribute__((address_space(3))) s16x4_t *)(lds_u8 *)(vp + 8 * RB)));
+                        vf[p] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+                    }
+                };
+                auto weigh = [&](int k, const uint4 (&vf)[NC], f32x16_t x) __attribute__((always_inline)) {
+                    if constexpr (F32) {
+                        x = pg_mfma32<OT>(vf[1], pf[k][0], x);
+                        x = pg_mfma32<OT>(vf[0], pf[k][1], x);
+                        return pg_mfma32<OT>(vf[0], pf[k][0], x);
+                    } else {
 #pragma unroll
-                            for (int p = NQ - 1; p >= 0; p--) x = pg_mfma32<OT>(vf[0], pf[p], x);
-                            return x;
-                        }
-                    };
-                    if (!wild) {
+                        for (int p = NQ - 1; p >= 0; p--) x = pg_mfma32<OT>(vf[0], pf[k][p], x);
+                        return x;
+                    }
+                };
 #pragma unroll
-                        for (int d = 0; d < ND; d++) {
-                            uint4 vf[NC];
-                            values(d, vf);
-                            o[d] = weigh(vf, o[d]);
-                        }
-                    } else {                     /* token by token, each from the values that it sees */
+                for (int k = 0; k < 2 * NB; k++)
+#pragma unroll
+                    for (int d = 0; d < ND; d++) {
+                        uint4 vf[NC];
+                        values(k, d, vf);
+                        o[d] = weigh(k, vf, o[d]);
+                    }
+                if (wild) {
+                    /* The rest, for the rows that see it, from the pages again: in memory, in the place
+                       that the item's piece may take when it is done, so that this seldom path
+                       holds no registers */
+                    const pg_args *la = pg_late_args();
+                    float4 *mine = (float4 *)((uint8_t *)la->pacc +
+                                              ((size_t)2 * me + (me == pg_owner(it.first, sh.U, W))) * P::SLOT) +
+                                   w * (ND * 256) + lane;
+#pragma unroll
+                    for (int i = 0; i < 4 * ND; i++)
+                        mine[64 * i] = make_float4(o[i >> 2][4 * (i & 3)], o[i >> 2][4 * (i & 3) + 1],
+                                                   o[i >> 2][4 * (i & 3) + 2], o[i >> 2][4 * (i & 3) + 3]);
 #pragma nounroll
-                        for (int z = wt0; z <= wt1; z++) {
-                            const int ph = first + z, pl = a.b.window > 0 ? ph - a.b.window + 1 : 0;
-                            const int jk = jb + 16 * k + 4 * h;
-                            auto seen = [&](int i) { return jk + i <= ph && jk + i >= pl; };
-                            uint32_t mask[4];
+                    for (int j = max(jb, klo); j < min(jb + KT, khi); j++) {
+                        const uint32_t vid = (uint32_t)ids[j >> a.b.plog];
+                        if (vid >= (uint32_t)a.n_pages) continue;
+                        const uint64_t vp = (uint64_t)vb + ((uint64_t)(vid * a.page_units + (uint32_t)(j & pmask) * a.slot_units) << a.ush);
+                        if (j > pos || j < pos_lo) continue;
+#pragma nounroll
+                        for (int i = 0; i < 4 * ND; i++) {
+                            float4 x = mine[64 * i];
+                            float *xs = &x.x;
 #pragma unroll
-                            for (int i = 0; i < 4; i++) {
-                                const int j = 8 * (i >> 1) + 2 * (i & 1);
-                                mask[i] = (seen(j) ? 0xFFFFu : 0u) | (seen(j + 1) ? 0xFFFF0000u : 0u);
+                            for (int k = 0; k < 4; k++) {
+                                const int e = 8 * i + 4 * h + k;
+                                float y;
+                                if constexpr (F32) y = pg_load<float>(vp + 4 * e);
+                                else y = pg_unpack2<CT>(pg_load<uint16_t>(vp + 2 * e)).x;
+                                xs[k] += fabsf(y) < INFINITY ? 0.0f : y;
                             }
-#pragma unroll
-                            for (int d = 0; d < ND; d++) {
-                                uint4 vf[NC];
-                                values(d, vf);
-#pragma unroll
-                                for (int p = 0; p < NC; p++)
-                                    vf[p] = make_uint4(vf[p].x & mask[0], vf[p].y & mask[1], vf[p].z & mask[2], vf[p].w & mask[3]);
-                                const f32x16_t x = weigh(vf, o[d]);
-#pragma unroll
-                                for (int i = 0; i < 16; i++) o[d][i] = tok == z ? x[i] : o[d][i];
-                            }
+                            mine[64 * i] = x;
                         }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4 * ND; i++) {
+                        const float4 x = mine[64 * i];
+                        o[i >> 2][4 * (i & 3)] = x.x;
+                        o[i >> 2][4 * (i & 3) + 1] = x.y;
+                        o[i >> 2][4 * (i & 3) + 2] = x.z;
+                        o[i >> 2][4 * (i & 3) + 3] = x.w;
                     }
                 }
             }
@@ -455,7 +489,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_paged_many(const pg_
         auto place = [&](int x) { return (size_t)2 * x + (x == wf); };
         auto finish = [&](float top, float L) __attribute__((always_inline)) {
             if (!row_ok) return;
-            const float nan = __int_as_float(0x7fc00000);
+            const float nan = __int_as_float(0x7fc00000), inv = __fdiv_rn(1.0f, L);
             float e = (top + __builtin_amdgcn_logf(ldexpf(L, -(int)P::LIFT))) * 0.69314718055994531f;
             const bool none = sq.p0 + t0 + tok < 0;
             if (sq.bad) e = nan;
@@ -465,7 +499,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_paged_many(const pg_
             for (int d = 0; d < ND; d++)
 #pragma unroll
                 for (int b = 0; b < 4; b++) {
-                    float4 y = make_float4(o[d][4 * b] / L, o[d][4 * b + 1] / L, o[d][4 * b + 2] / L, o[d][4 * b + 3] / L);
+                    float4 y = make_float4(o[d][4 * b] * inv, o[d][4 * b + 1] * inv, o[d][4 * b + 2] * inv, o[d][4 * b + 3] * inv);
                     if (sq.bad) y = make_float4(nan, nan, nan, nan);
                     else if (none) y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                     pg_put4<AT>(late->out, qrow * late->ldo + (size_t)qh * HD + 32 * d + 8 * b + 4 * h, y);
@@ -476,9 +510,8 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_paged_many(const pg_
             continue;
         }
         /* a piece: per slot the four wavefronts' blocks of 4 ND x 64 lanes x 16 bytes */
-        constexpr size_t SLOT = (size_t)PG_MANY_ROWS * HD * 4;
         auto put = [&](size_t slot, float top, float L) __attribute__((always_inline)) {
-            uint8_t *pa = (uint8_t *)late->pacc + slot * SLOT + (size_t)w * (ND * 4096);
+            uint8_t *pa = (uint8_t *)late->pacc + slot * P::SLOT + (size_t)w * (ND * 4096);
 #pragma unroll
             for (int d = 0; d < ND; d++)
 #pragma unroll
@@ -500,7 +533,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_paged_many(const pg_
 #pragma nounroll
             for (int k = 0; k < n; k++) {
                 const size_t slot = place(x0 + k * step);
-                const uint8_t *pa = (const uint8_t *)late->pacc + slot * SLOT + (size_t)w * (ND * 4096);
+                const uint8_t *pa = (const uint8_t *)late->pacc + slot * P::SLOT + (size_t)w * (ND * 4096);
                 const unsigned long long mb = ld_agent((const unsigned long long *)(late->pml + slot * PG_MANY_ROWS + 32 * w + c));
                 v4i_t y[ND][4];
 #pragma unroll
