@@ -43,9 +43,10 @@ template <int CT, int AT, int HD> struct pg_many_t {
     static constexpr int RB = 2 * HDP, CPR = RB / 16;            /* an LDS row: bytes, chunks */
     static constexpr int PLANE = KT * RB, BUF = 2 * NC * PLANE;  /* K planes, V planes */
     static constexpr int NB = KT / 32, NS = HD / 16, ND = HD / 32;
-    /* 16-bit: copies of 1 KiB per wavefront and step, and rows in each. f32: chunks per thread */
-    static constexpr int CHUNKS = KT * (HD / 8);
-    static constexpr int E = F32 ? (CHUNKS + 255) / 256 : PLANE / 4096, RPE = 64 / CPR;
+    /* a wavefront stages RW consecutive rows. 16-bit: E copies of 1 KiB, RPE rows each; f32: E chunks
+       of eight elements to a lane, of CHUNKS */
+    static constexpr int RW = KT / 4, CHUNKS = RW * (HD / 8);
+    static constexpr int E = F32 ? (CHUNKS + 63) / 64 : PLANE / 4096, RPE = 64 / CPR;
     static constexpr size_t SLOT = (size_t)PG_MANY_ROWS * HD * 4;  /* bytes of a piece */
     static constexpr float LIFT = OT == CPG_T_F16 ? 4.0f : 0.0f;
     __host__ __device__ static constexpr int kswz(int r) { return CPR == 8 ? (r >> 1) & 7 : r & 15; }
@@ -140,66 +141,77 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_paged_many(const pg_
         const uint8_t *kb = a.k + (size_t)it.kv * a.head_bytes;
         const uint8_t *vb = a.v + (size_t)it.kv * a.head_bytes;
 
-        /* ---- staging. Copy (16-bit) or chunk (f32) e of a step: its row of the step, and the
-           chunk of it that goes to the lane's place */
-        auto row_e = [&](int e) __attribute__((always_inline)) {
-            return F32 ? min(tid + 256 * e, P::CHUNKS - 1) / (HD / 8) : (w * E + e) * P::RPE + lane / CPR;
+        /* ---- staging. Copy (16-bit) or chunk (f32) e of a step: its row among the wavefront's, and
+           the place of its 16 bytes (32 of an f32 cache) in rows of keys and of values */
+        auto chunk_e = [&](int e) { return min(lane + 64 * e, P::CHUNKS - 1); };
+        auto row_e = [&](int e) { return F32 ? chunk_e(e) / (HD / 8) : e * P::RPE + lane / CPR; };
+        auto kcol = [&](int e) {
+            return F32 ? 32 * (chunk_e(e) % (HD / 8)) : 16 * min((lane % CPR) ^ P::kswz(P::RW * w + row_e(e)), HD / 8 - 1);
         };
-        /* the row of the step that lane l % KT finds for all: the page of its key, in another register
-           while that flies, and the row's offset. A key that no row sees stands for one that does
-           (its score is masked; should its value be no number, that is noted below) */
-        auto key_of = [&](int n) { return max(min(max(j0 + KT * n + lane % KT, klo), khi - 1), 0); };
+        auto vcol = [&](int e) {
+            return F32 ? 32 * (chunk_e(e) % (HD / 8)) : 16 * min((lane % CPR) ^ P::vswz(P::RW * w + row_e(e)), HD / 8 - 1);
+        };
+        /* A key that no row sees stands for one that does (its score is masked; should its value be no
+           number, that is noted below). Where a wavefront's rows lie in one page (`flat`), its id is
+           one number and the rows' places in it are the same in every step. */
+        const bool flat = (1 << a.b.plog) >= P::RW && (uint64_t)a.slot_units << a.ush < (uint64_t)1 << 26;
+        auto key_of = [&](int n) {
+            return max(min(max(j0 + KT * n + P::RW * w + (flat ? 0 : lane % P::RW), klo), khi - 1), 0);
+        };
         auto load_id = [&](int n) { return ids[key_of(n) >> a.b.plog]; };
-        uint32_t ro;
-        bool lost;                               /* a bad page id among the step's */
-        auto make_rows = [&](int n, int id) __attribute__((always_inline)) {
-            const bool miss = (uint32_t)id >= (uint32_t)a.n_pages;
-            ro = (uint32_t)id * a.page_units + (uint32_t)(key_of(n) & pmask) * a.slot_units;
-            lost = __any(miss);
-            if (lost) {
-                ro = miss ? PG_BAD_ROW : ro;
-                if (lane == 0 && khi > 0) *pg_late_args()->stat = 1;     /* no key: no page is needed */
+        uint32_t koff[E], voff[E];
+        {
+            const uint32_t slot_bytes = a.slot_units << a.ush;
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                koff[e] = row_e(e) * slot_bytes + kcol(e);
+                voff[e] = row_e(e) * slot_bytes + vcol(e);
             }
-        };
-        /* the addresses of row i of the step: of its key (a bad page's: NaN, and its scores with it)
-           and of its value */
-        auto rows_at = [&](int i, uint64_t &kp, uint64_t &vp) __attribute__((always_inline)) {
-            const uint32_t r = __shfl(ro, i);
-            const uint64_t off = (uint64_t)r << a.ush;
-            kp = (uint64_t)kb + off;
-            vp = (uint64_t)vb + off;
-            if (lost && r == PG_BAD_ROW) {
-                kp = (uint64_t)a.blank + 1024;
-                vp = (uint64_t)a.blank;
+        }
+        /* put(e, key's base, its offset, value's base, its offset) for the wavefront's rows of step n */
+        auto stage = [&](int n, int id, auto put) __attribute__((always_inline)) {
+            const int one = __builtin_amdgcn_readfirstlane(id);
+            if (flat && (uint32_t)one < (uint32_t)a.n_pages) {
+                const int j = j0 + KT * n + P::RW * w;
+                const uint64_t off = (uint64_t)((uint32_t)one * a.page_units + (uint32_t)(j & pmask) * a.slot_units) << a.ush;
+#pragma unroll
+                for (int e = 0; e < E; e++) put(e, kb + off, koff[e], vb + off, voff[e]);
+                return;
+            }
+            const int j = flat ? j0 + KT * n + P::RW * w + lane % P::RW : key_of(n);
+            const bool miss = (uint32_t)id >= (uint32_t)a.n_pages;       /* the key NaN, and its scores */
+            if (__any(miss) && lane == 0 && khi > 0) *pg_late_args()->stat = 1;    /* no key: no page is needed */
+            const uint32_t ro = miss ? PG_BAD_ROW : (uint32_t)id * a.page_units + (uint32_t)(j & pmask) * a.slot_units;
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                const uint32_t r = __shfl(ro, row_e(e));
+                put(e, nullptr, pg_row_ptr(kb, r, a.ush, a.blank, true) + kcol(e), nullptr,
+                    pg_row_ptr(vb, r, a.ush, a.blank, false) + vcol(e));
             }
         };
         const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_u8 *)lds;
-        auto copy = [&](int buf) __attribute__((always_inline)) {
-#pragma unroll
-            for (int e = 0; e < E; e++) {
-                const int r = row_e(e), pc = lane % CPR;
-                const uint32_t dst = lds0 + buf * P::BUF + (w * E + e) * 1024;
-                const int kc = min(pc ^ P::kswz(r), HD / 8 - 1), vc = min(pc ^ P::vswz(r), HD / 8 - 1);
-                uint64_t kp, vp;
-                rows_at(r, kp, vp);
-                pg_dma16(kp + 16 * kc, dst);
-                pg_dma16(vp + 16 * vc, dst + P::PLANE);
-            }
+        auto copy = [&](int n, int id, int buf) __attribute__((always_inline)) {
+            const uint32_t to = lds0 + buf * P::BUF + w * E * 1024;
+            stage(n, id, [&](int e, const uint8_t *kp, auto ko, const uint8_t *vp, auto vo) __attribute__((always_inline)) {
+                if constexpr (sizeof(ko) == 4) {
+                    lds_dma16(kp, ko, to + e * 1024);
+                    lds_dma16(vp, vo, to + e * 1024 + P::PLANE);
+                } else {
+                    pg_dma16(ko, to + e * 1024);
+                    pg_dma16(vo, to + e * 1024 + P::PLANE);
+                }
+            });
         };
         constexpr int EF = F32 ? E : 1;
         u32x4_t kraw[EF][2], vraw[EF][2];
-        auto fetch = [&]() __attribute__((always_inline)) {
-#pragma unroll
-            for (int e = 0; e < EF; e++) {
-                const uint64_t d = 32 * (min(tid + 256 * e, P::CHUNKS - 1) % (HD / 8));
-                uint64_t kp, vp;
-                rows_at(row_e(e), kp, vp);
+        auto fetch = [&](int n, int id) __attribute__((always_inline)) {
+            stage(n, id, [&](int e, const uint8_t *kp, auto ko, const uint8_t *vp, auto vo) __attribute__((always_inline)) {
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
-                    kraw[e][i] = pg_load<u32x4_t>(kp + d + 16 * i);
-                    vraw[e][i] = pg_load<u32x4_t>(vp + d + 16 * i);
+                    kraw[e][i] = pg_load<u32x4_t>((uint64_t)kp + ko + 16 * i);
+                    vraw[e][i] = pg_load<u32x4_t>((uint64_t)vp + vo + 16 * i);
                 }
-            }
+            });
         };
         auto split_to = [&](uint8_t *dst, const u32x4_t (&x)[2]) __attribute__((always_inline)) {
             uint32_t hi[4], lo[4];
@@ -217,7 +229,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_paged_many(const pg_
 #pragma unroll
             for (int e = 0; e < EF; e++) {
                 /* past the last chunk: the last one again, the same bytes */
-                const int r = row_e(e), ch = min(tid + 256 * e, P::CHUNKS - 1) % (HD / 8);
+                const int r = P::RW * w + row_e(e), ch = chunk_e(e) % (HD / 8);
                 uint8_t *b = lds + buf * P::BUF + r * RB;
                 split_to(b + ((ch ^ P::kswz(r)) << 4), kraw[e]);
                 split_to(b + NC * P::PLANE + ((ch ^ P::vswz(r)) << 4), vraw[e]);
@@ -297,14 +309,13 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_paged_many(const pg_
             }
         }
         /* the first step into buffer 0 */
-        make_rows(0, id);
         if constexpr (F32) {
-            fetch();
+            fetch(0, id);
             id = load_id(1);
             note(0, 0, turn);
             store(0);
         } else {
-            copy(0);
+            copy(0, id, 0);
             id = load_id(1);
             wait_vm_lgkm<0>();
             note(0, 0, turn);
@@ -320,32 +331,38 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_paged_many(const pg_
             const int jb = j0 + KT * n, buf = n & 1;
             const bool more = n + 1 < steps;
             if (more) {
-                make_rows(n + 1, id);
-                if constexpr (F32) fetch();
-                else copy(buf ^ 1);
+                if constexpr (F32) fetch(n + 1, id);
+                else copy(n + 1, id, buf ^ 1);
                 id = load_id(n + 2);
             }
             if (active && jb <= wlast && jb + KT > wklo) {
                 const uint8_t *base = lds + buf * P::BUF;
                 /* scores: st[b][i] of key jb + 32 b + 8 (i / 4) + 4 h + i % 4 */
+                /* The order of reads and products is fenced throughout: left alone the compiler reads an
+                   operand and waits for it at once. Operand t of the keys: block t % NB, elements
+                   16 (t / NB) ..; PD of them are read ahead of the products. */
                 f32x16_t st[NB];
-#pragma unroll
-                for (int b = 0; b < NB; b++) {
-                    st[b] = f32x16_t{};
-#pragma unroll
-                    for (int i = 0; i < NS; i++) {
-                        uint4 kf[NC];
+                {
+                    constexpr int NT = NS * NB, PD = NQ > 1 ? 2 : 4;
+                    uint4 kf[PD][NC];
+                    auto read = [&](int t) __attribute__((always_inline)) {
 #pragma unroll
                         for (int p = 0; p < NC; p++)
-                            kf[p] = *(const uint4 *)(base + p * P::PLANE + 32 * b * RB + (kread ^ (i << 5)));
-                        if constexpr (F32) {
-                            st[b] = pg_mfma32<OT>(kf[1], qf[0][i], st[b]);
-                            st[b] = pg_mfma32<OT>(kf[0], qf[1][i], st[b]);
-                            st[b] = pg_mfma32<OT>(kf[0], qf[0][i], st[b]);
-                        } else {
+                            kf[t % PD][p] = *(const uint4 *)(base + p * P::PLANE + 32 * (t % NB) * RB + (kread ^ (t / NB << 5)));
+                    };
 #pragma unroll
-                            for (int p = NQ - 1; p >= 0; p--) st[b] = pg_mfma32<OT>(kf[0], qf[p][i], st[b]);
-                        }
+                    for (int t = 0; t < PD; t++) read(t);
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int t = 0; t < NT; t++) {
+                        const uint4 (&k)[NC] = kf[t % PD];
+                        f32x16_t &x = st[t % NB];
+                        if (t < NB) x = f32x16_t{};
+                        if constexpr (F32) x = pg_mfma32<OT>(k[1], qf[0][t / NB], x);
+#pragma unroll
+                        for (int p = NQ - 1; p >= 0; p--) x = pg_mfma32<OT>(k[0], qf[p][t / NB], x);
+                        if (t + PD < NT) read(t + PD);
+                        __builtin_amdgcn_sched_barrier(0);
                     }
                 }
                 const bool edge = jb < wfull || jb + KT - 1 > wfirst;
@@ -376,53 +393,57 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_paged_many(const pg_
                 }
                 const float off = P::LIFT - (M == -INFINITY ? 0.0f : M);
                 const bool wild = crosses(n) && wild_s[turn & 3] != 0;
-                /* the weights, 16 keys to an operand */
-                uint4 pf[2 * NB][NQ];
+                /* The weights of 16 keys are an operand, computed among the products of the 16 before.
+                   Operand t of the values: keys 16 (t / ND) .., elements 32 (t % ND) .. */
+                {
+                    constexpr int NT = 2 * NB * ND, PD = NQ > 1 ? 2 : 4;
+                    uint4 vf[PD][NC], pf[2][NQ];
+                    auto read = [&](int t) __attribute__((always_inline)) {
 #pragma unroll
-                for (int k = 0; k < 2 * NB; k++) {
-                    uint32_t wd[4][NQ];
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
+                        for (int p = 0; p < NC; p++) {
+                            const uint8_t *vp = base + p * P::PLANE + 16 * (t / ND) * RB + (vread ^ (t % ND << 6));
+                            const uint2 lo = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                (__attribute__((address_space(3))) s16x4_t *)(lds_u8 *)vp));
+                            const uint2 hi = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                (__attribute__((address_space(3))) s16x4_t *)(lds_u8 *)(vp + 8 * RB)));
+                            vf[t % PD][p] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+                        }
+                    };
+                    /* word i (of 4) of the weights of keys 16 k .. */
+                    auto weight = [&](int k, int i) __attribute__((always_inline)) {
                         const float x = __builtin_amdgcn_exp2f(fmaf(st[k >> 1][8 * (k & 1) + 2 * i], cs, off));
                         const float y = __builtin_amdgcn_exp2f(fmaf(st[k >> 1][8 * (k & 1) + 2 * i + 1], cs, off));
                         l += x;
                         l += y;
-                        pg_pieces2<OT, NQ>(x, y, wd[i]);
-                    }
+                        uint32_t wd[NQ];
+                        pg_pieces2<OT, NQ>(x, y, wd);
 #pragma unroll
-                    for (int p = 0; p < NQ; p++) pf[k][p] = make_uint4(wd[0][p], wd[1][p], wd[2][p], wd[3][p]);
+                        for (int p = 0; p < NQ; p++) {
+                            if (i == 0) pf[k & 1][p].x = wd[p];
+                            if (i == 1) pf[k & 1][p].y = wd[p];
+                            if (i == 2) pf[k & 1][p].z = wd[p];
+                            if (i == 3) pf[k & 1][p].w = wd[p];
+                        }
+                    };
+#pragma unroll
+                    for (int t = 0; t < PD; t++) read(t);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) weight(0, i);
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int t = 0; t < NT; t++) {
+                        const int k = t / ND, d = t % ND;
+                        const uint4 (&v)[NC] = vf[t % PD];
+                        if constexpr (F32) o[d] = pg_mfma32<OT>(v[1], pf[k & 1][0], o[d]);
+#pragma unroll
+                        for (int p = NQ - 1; p >= 0; p--) o[d] = pg_mfma32<OT>(v[0], pf[k & 1][p], o[d]);
+                        if (t + PD < NT) read(t + PD);
+                        if (k + 1 < 2 * NB)
+#pragma unroll
+                            for (int i = 4 * d / ND; i < 4 * (d + 1) / ND; i++) weight(k + 1, i);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
                 }
-                /* elements 32 d .. of the values of keys 16 k .. */
-                auto values = [&](int k, int d, uint4 (&vf)[NC]) __attribute__((always_inline)) {
-#pragma unroll
-                    for (int p = 0; p < NC; p++) {
-                        const uint8_t *vp = base + p * P::PLANE + 16 * k * RB + (vread ^ (d << 6));
-                        const uint2 lo = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                            (__attribute__((address_space(3))) s16x4_t *)(lds_u8 *)vp));
-                        const uint2 hi = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                            (__attribute__((address_space(3))) s16x4_t *)(lds_u8 *)(vp + 8 * RB)));
-                        vf[p] = make_uint4(lo.x, lo.y, hi.x, hi.y);
-                    }
-                };
-                auto weigh = [&](int k, const uint4 (&vf)[NC], f32x16_t x) __attribute__((always_inline)) {
-                    if constexpr (F32) {
-                        x = pg_mfma32<OT>(vf[1], pf[k][0], x);
-                        x = pg_mfma32<OT>(vf[0], pf[k][1], x);
-                        return pg_mfma32<OT>(vf[0], pf[k][0], x);
-                    } else {
-#pragma unroll
-                        for (int p = NQ - 1; p >= 0; p--) x = pg_mfma32<OT>(vf[0], pf[k][p], x);
-                        return x;
-                    }
-                };
-#pragma unroll
-                for (int k = 0; k < 2 * NB; k++)
-#pragma unroll
-                    for (int d = 0; d < ND; d++) {
-                        uint4 vf[NC];
-                        values(k, d, vf);
-                        o[d] = weigh(k, vf, o[d]);
-                    }
                 if (wild) {
                     /* The rest, for the rows that see it, from the pages again: in memory, in the place
                        that the item's piece may take when it is done, so that this seldom path
@@ -464,6 +485,10 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_paged_many(const pg_
                         o[i >> 2][4 * (i & 3) + 2] = x.z;
                         o[i >> 2][4 * (i & 3) + 3] = x.w;
                     }
+                    /* waited for here: where the paths join it would be in every step, and for the
+                       copies in flight too */
+#pragma unroll
+                    for (int d = 0; d < ND; d++) asm volatile("" : "+v"(o[d]));
                 }
             }
             if (more) {
