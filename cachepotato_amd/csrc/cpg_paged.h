@@ -19,7 +19,8 @@ struct pg_args {
     const int *pages;
     pg_batch b;
     int64_t ldq, head_bytes;
-    int H, G, n_pages, hpp; /* hpp: query heads per tile */
+    int H, G, n_pages;
+    int hpp, hinv;          /* query heads per tile; 2^16 / hpp rounded up: r hinv >> 16 = r / hpp for r < 128 */
     uint32_t page_units, slot_units;
     int ush;
     float scale2;           /* scale * log2(e) */

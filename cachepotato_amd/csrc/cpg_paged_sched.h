@@ -22,10 +22,11 @@
 #define PG_MAX_LEN (1 << 30) /* tokens of a sequence: positions and their sums stay in 32 bits */
 
 /* the batch and its division: S sequences, T rows; parts of a kv head's query heads; log2 of the
-   tokens of a page, of those of a tile and of the keys of a unit (tl <= ul) */
+   tokens of a page, of those of a tile and of the keys of a unit (tl <= ul); the units that an item
+   counts for ahead of its keys (its start and its end take the time of some) */
 struct pg_batch {
     const int *q_off, *len;
-    int S, T, KV, max_pages, plog, window, parts, tl, ul;
+    int S, T, KV, max_pages, plog, window, parts, tl, ul, extra;
 };
 
 PG_FN int pg_min(int a, int b) { return a < b ? a : b; }
@@ -66,14 +67,15 @@ PG_FN int pg_unit_lo(const pg_batch &b, const pg_seq &s, int i) {
 /* units of the tiles before tile x of a sequence (every tile has one at least, so that the rows
    without a key are written too): with the position of a tile's last row a_i = p0 + (i + 1) TB - 1,
    the sum of floor(a_i / UNIT) + 1 - floor(b_i / UNIT) over the tiles with a key, b_i the first key
-   that the tile's first row sees, in closed form since TB divides UNIT */
+   that the tile's first row sees, in closed form since TB divides UNIT; and `extra` for each tile */
 PG_FN uint32_t pg_units_before(const pg_batch &b, const pg_seq &s, int x) {
     const int nt = pg_tiles(s, b.tl), tl = b.tl;
     const int i0 = s.len <= 0 ? nt : s.p0 >= 0 ? 0 : (-s.p0) >> tl;   /* first tile with a key */
-    if (x <= i0) return (uint32_t)x;
+    const uint32_t more = (uint32_t)x * (uint32_t)b.extra;
+    if (x <= i0) return (uint32_t)x + more;
     const int c = x - i0, k = b.ul - tl;
     const int A = (s.p0 + ((i0 + 1) << tl) - 1) >> tl;
-    uint32_t sum = (uint32_t)x + pg_floor_sum(A + c, k) - pg_floor_sum(A, k);
+    uint32_t sum = (uint32_t)x + more + pg_floor_sum(A + c, k) - pg_floor_sum(A, k);
     if (x == nt)                                 /* the last tile may be short */
         sum += (uint32_t)(((s.p0 + s.n - 1) >> b.ul) - ((A + c - 1) >> k));
     if (b.window > 0) {
@@ -125,9 +127,11 @@ PG_FN int pg_owner(uint32_t u, uint32_t U, int W) {
 /* a walk over a share's items */
 struct pg_item {
     int kv, part, tile;     /* the item */
-    int off, cnt;           /* its units from `off` on, cnt of them, are this workgroup's */
-    int all;                /* its units */
-    uint32_t first;         /* the number of its first unit among all */
+    int step;               /* units to go on by */
+    int off, cnt;           /* its units of keys from `off` on, cnt of them, are this workgroup's; none
+                               where the share ends in the units ahead of the keys */
+    int all;                /* its units of keys */
+    uint32_t first;         /* the number of its first unit of keys among all units */
 };
 
 /* the item of sequence q at unit u (below u1, `rem` units into the sequence) */
@@ -146,10 +150,12 @@ PG_FN pg_item pg_find_item(const pg_batch &b, const pg_seq &q, uint32_t u, uint3
         else { hi = mid; upto = x; }
     }
     it.tile = lo;
-    it.all = (int)(upto - ahead);
-    it.off = (int)(in - ahead);
-    it.first = u - it.off;
-    it.cnt = pg_min(it.all - it.off, (int)(u1 - u));
+    const int at = (int)(in - ahead);            /* of the item's units, those ahead of the keys first */
+    it.step = pg_min((int)(upto - ahead) - at, (int)(u1 - u));
+    it.all = (int)(upto - ahead) - b.extra;
+    it.off = pg_max(at - b.extra, 0);
+    it.cnt = at + it.step - b.extra - it.off;
+    it.first = u - at + b.extra;
     return it;
 }
 

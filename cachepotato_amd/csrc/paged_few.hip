@@ -94,16 +94,18 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_paged_few(const pg_a
     const int W = sh.W, me = sh.w;
     int s = at.s;
     uint32_t rem = at.rem;
+    pg_seq sq = pg_get_seq(a.b.q_off, a.b.len, s, a.b.T, a.b.max_pages, a.b.plog);
     for (uint32_t u = sh.u0; u < sh.u1;) {
-        const pg_seq sq = pg_get_seq(a.b.q_off, a.b.len, s, a.b.T, a.b.max_pages, a.b.plog);
         if (rem >= pg_seq_units(a.b, sq)) {      /* the sequence is done, or brings nothing */
             s++;
             rem = 0;
+            sq = pg_get_seq(a.b.q_off, a.b.len, s, a.b.T, a.b.max_pages, a.b.plog);
             continue;
         }
         const pg_item it = pg_find_item(a.b, sq, u, sh.u1, rem);
-        u += it.cnt;
-        rem += it.cnt;
+        u += it.step;
+        rem += it.step;
+        if (it.cnt <= 0) continue;               /* its keys are all the next workgroups' */
         /* the thread's number is made opaque, here and behind the loop: what follows from it would
            else be computed ahead of the walk and held, or spilled, over everything */
         int lane = tid & 63;
@@ -111,7 +113,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_paged_few(const pg_a
         const int c = lane & 15, g = lane >> 4;
         /* the lane's query: row c of the tile */
         const int t0 = it.tile << a.b.tl, tb = min(1 << a.b.tl, sq.n - t0);
-        const int tok = c / a.hpp, hq = it.part * a.hpp + c - tok * a.hpp;
+        const int tok = c * a.hinv >> 16, hq = it.part * a.hpp + c - tok * a.hpp;
         const bool row_ok = tok < tb && hq < a.G;
         const int pos = row_ok ? sq.p0 + t0 + tok : -1;           /* keys pos_lo .. pos */
         const int pos_lo = a.b.window > 0 ? max(0, pos - a.b.window + 1) : 0;
@@ -373,7 +375,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_paged_few(const pg_a
         const size_t slot = ((size_t)2 * me + (me == wf)) * PG_FEW_ROWS;
         /* the finished row: divided, or zeros where it has no key, or NaN where the batch is bad */
         auto finish = [&](int r, int d, float4 v, float top, float L) __attribute__((always_inline)) {
-            const int rt = r / a.hpp, rh = it.part * a.hpp + r - rt * a.hpp;
+            const int rt = r * a.hinv >> 16, rh = it.part * a.hpp + r - rt * a.hpp;
             if (rh >= a.G) return;
             const int rp = sq.p0 + t0 + rt, h = it.kv * a.G + rh;
             const size_t row = (size_t)(sq.lo + t0 + rt);

@@ -103,23 +103,25 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_paged_many(const pg_
     if (tid < 4) wild_s[tid] = 0;
     __syncthreads();
     int turn = 0;                                /* steps so far */
+    pg_seq sq = pg_get_seq(a.b.q_off, a.b.len, s, a.b.T, a.b.max_pages, a.b.plog);
     for (uint32_t u = sh.u0; u < sh.u1;) {
-        const pg_seq sq = pg_get_seq(a.b.q_off, a.b.len, s, a.b.T, a.b.max_pages, a.b.plog);
         if (rem >= pg_seq_units(a.b, sq)) {      /* the sequence is done, or brings nothing */
             s++;
             rem = 0;
+            sq = pg_get_seq(a.b.q_off, a.b.len, s, a.b.T, a.b.max_pages, a.b.plog);
             continue;
         }
         const pg_item it = pg_find_item(a.b, sq, u, sh.u1, rem);
-        u += it.cnt;
-        rem += it.cnt;
+        u += it.step;
+        rem += it.step;
+        if (it.cnt <= 0) continue;               /* its keys are all the next workgroups' */
         /* opaque, as in k_paged_few: nothing that follows from it is held over the walk */
         int lane = tid & 63;
         asm volatile("" : "+v"(lane));
         const int c = lane & 31, h = lane >> 5;
         /* the lane's query: row 32 w + c of the tile */
         const int t0 = it.tile << a.b.tl, tb = min(1 << a.b.tl, sq.n - t0);
-        const int row = 32 * w + c, tok = row / a.hpp, hq = it.part * a.hpp + row - tok * a.hpp;
+        const int row = 32 * w + c, tok = row * a.hinv >> 16, hq = it.part * a.hpp + row - tok * a.hpp;
         const bool row_ok = tok < tb && hq < a.G;
         const int pos = row_ok ? sq.p0 + t0 + tok : -1;              /* keys pos_lo .. pos */
         const int pos_lo = a.b.window > 0 ? max(0, pos - a.b.window + 1) : 0;
@@ -128,7 +130,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_paged_many(const pg_
         /* positions of the tile, and of the wavefront's rows */
         const int first = sq.p0 + t0, last = first + tb - 1;
         const int klo = a.b.window > 0 ? max(0, first - a.b.window + 1) : 0, khi = last + 1;
-        const int wt0 = 32 * w / a.hpp, wt1 = min((32 * w + 31) / a.hpp, tb - 1);
+        const int wt0 = 32 * w * a.hinv >> 16, wt1 = min((32 * w + 31) * a.hinv >> 16, tb - 1);
         const bool active = wt0 < tb;
         const int wfirst = first + wt0, wlast = first + wt1;
         const int wklo = a.b.window > 0 ? max(0, wfirst - a.b.window + 1) : 0;
@@ -269,6 +271,10 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_paged_many(const pg_
         float M = -INFINITY, l = 0.0f;           /* what the weights refer to, in log2; -inf: nothing yet */
 
         int id = load_id(0);
+        /* the first step into buffer 0, and the queries behind its loads */
+        if constexpr (F32) fetch(0, id);
+        else copy(0, id, 0);
+        id = load_id(1);
         /* ---- the queries */
         uint4 qf[NQ][NS];
         float cs = a.scale2;
@@ -308,15 +314,10 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_paged_many(const pg_
                 }
             }
         }
-        /* the first step into buffer 0 */
         if constexpr (F32) {
-            fetch(0, id);
-            id = load_id(1);
             note(0, 0, turn);
             store(0);
         } else {
-            copy(0, id, 0);
-            id = load_id(1);
             wait_vm_lgkm<0>();
             note(0, 0, turn);
         }

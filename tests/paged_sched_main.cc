@@ -33,9 +33,9 @@ static int count_units(const pg_batch &b, const pg_seq &s, int i, int *lo_unit) 
 }
 
 static int check(const std::vector<int> &off, const std::vector<int> &len, int T, int KV, int parts, int tl,
-                 int ul, int window, int plog, int max_pages, int grid) {
+                 int ul, int extra, int window, int plog, int max_pages, int grid) {
     const int S = (int)len.size();
-    const pg_batch b = {off.data(), len.data(), S, T, KV, max_pages, plog, window, parts, tl, ul};
+    const pg_batch b = {off.data(), len.data(), S, T, KV, max_pages, plog, window, parts, tl, ul, extra};
     int64_t U = 0;
     std::vector<int64_t> before(S);
     for (int s = 0; s < S; s++) {
@@ -55,7 +55,7 @@ static int check(const std::vector<int> &off, const std::vector<int> &len, int T
                 printf("first unit of tile %d\n", i);
                 return 1;
             }
-            sum += c;
+            sum += c + extra;
         }
         if (pg_seq_units(b, q) != sum * KV * parts) { printf("units of %d\n", s); return 1; }
         before[s] = U;
@@ -89,8 +89,10 @@ static int check(const std::vector<int> &off, const std::vector<int> &len, int T
                 rem = 0;
             }
             const pg_item it = pg_find_item(b, q, u, r.u1, (uint32_t)rem);
-            rem += it.cnt;
-            if (it.cnt <= 0 || it.off < 0 || it.off + it.cnt > it.all || u + it.cnt > r.u1) { printf("bad item\n"); return 1; }
+            rem += it.step;
+            if (it.step <= 0 || it.off < 0 || it.off + it.cnt > it.all || u + it.step > r.u1) { printf("bad item\n"); return 1; }
+            u += it.step;
+            if (it.cnt <= 0) continue;
             auto key = std::make_tuple(s, it.kv, it.part, it.tile);
             if (!met.count(key)) firsts[key] = it.first;
             if (firsts[key] != it.first || (int)met[key].size() != it.off) { printf("pieces out of order\n"); return 1; }
@@ -101,7 +103,6 @@ static int check(const std::vector<int> &off, const std::vector<int> &len, int T
                 for (int i = 1; i < it.all; i++) pieces += met[key][i] != met[key][i - 1];
                 if (wf != met[key][0] || wl != w || wl - wf + 1 != pieces) { printf("owners %d..%d, met %d..%d\n", wf, wl, met[key][0], w); return 1; }
             }
-            u += it.cnt;
         }
     }
     if (next != U) { printf("%lld of %lld units dealt\n", (long long)next, (long long)U); return 1; }
@@ -143,19 +144,19 @@ int main() {
             else off[s + 1] = below(2) ? -5 : T + 7;
         }
         const int window = below(2) ? 0 : 1 + below(below(2) ? 20 : 500);
-        if (check(off, len, T, 1 + below(4), 1 + below(2), tl, tl + below(9 - tl), window, plog, max_pages, grids[below(7)])) {
+        if (check(off, len, T, 1 + below(4), 1 + below(2), tl, tl + below(9 - tl), below(2) ? 0 : below(5), window, plog, max_pages, grids[below(7)])) {
             printf("case %d\n", c);
             return 1;
         }
     }
     /* the largest positions: a sum that leaves 32 bits, differences that do not */
     const pg_seq big = {0, 1 << 10, PG_MAX_LEN, PG_MAX_LEN - (1 << 10), false, false};
-    const pg_batch b = {nullptr, nullptr, 1, 1 << 10, 1, 0, 0, 0, 1, 0, 12};
+    const pg_batch b = {nullptr, nullptr, 1, 1 << 10, 1, 0, 0, 0, 1, 0, 12, 1};
     uint32_t sum = 0;
     for (int i = 0; i < 1 << 10; i++) {
         int lo;
         if (pg_units_before(b, big, i) != sum) return 1;
-        sum += count_units(b, big, i, &lo);
+        sum += count_units(b, big, i, &lo) + 1;
     }
     printf("ok\n");
     return 0;
