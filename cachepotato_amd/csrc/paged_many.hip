@@ -339,9 +339,11 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_paged_many(const pg_
             if (active && jb <= wlast && jb + KT > wklo) {
                 const uint8_t *base = lds + buf * P::BUF;
                 /* scores: st[b][i] of key jb + 32 b + 8 (i / 4) + 4 h + i % 4 */
-                /* The order of reads and products is fenced throughout: left alone the compiler reads an
+                /* The matrix phases have the priority over the other workgroup's vector phases (2 %). The
+                   order of reads and products is fenced throughout: left alone the compiler reads an
                    operand and waits for it at once. Operand t of the keys: block t % NB, elements
                    16 (t / NB) ..; PD of them are read ahead of the products. */
+                __builtin_amdgcn_s_setprio(1);
                 f32x16_t st[NB];
                 {
                     constexpr int NT = NS * NB, PD = NQ > 1 ? 2 : 4;
@@ -366,6 +368,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_paged_many(const pg_
                         __builtin_amdgcn_sched_barrier(0);
                     }
                 }
+                __builtin_amdgcn_s_setprio(0);
                 const bool edge = jb < wfull || jb + KT - 1 > wfirst;
                 if (edge)
 #pragma unroll
@@ -431,6 +434,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_paged_many(const pg_
 #pragma unroll
                     for (int i = 0; i < 4; i++) weight(0, i);
                     __builtin_amdgcn_sched_barrier(0);
+                    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
                     for (int t = 0; t < NT; t++) {
                         const int k = t / ND, d = t % ND;
@@ -445,6 +449,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_paged_many(const pg_
                         __builtin_amdgcn_sched_barrier(0);
                     }
                 }
+                __builtin_amdgcn_s_setprio(0);
                 if (wild) {
                     /* The rest, for the rows that see it, from the pages again: in memory, in the place
                        that the item's piece may take when it is done, so that this seldom path
