@@ -7,7 +7,10 @@
 #include "cpg_paged_sched.h"
 
 #define PG_FEW_ROWS 16      /* query rows of a tile of k_paged_few: one MFMA tile */
-#define PG_FEW_WGS 512      /* workgroups of k_paged_few at most: two per CU */
+#define PG_FEW_WGS 256      /* workgroups of k_paged_few at most: one per CU. Its four wavefronts keep
+                               64 KiB in flight, and an item has half the pieces of two per CU: 16
+                               conversations 20.4 -> 18.6 us, one token over 32767 26.3 -> 21.9, 96
+                               sequences 212 -> 200 */
 #define PG_MANY_ROWS 128    /* query rows of a tile of k_paged_many: 32 to a wavefront */
 #define PG_MANY_WGS 512     /* workgroups of k_paged_many at most: two per CU */
 
@@ -31,7 +34,7 @@ struct pg_args {
     int64_t ldo;
     float *pacc;            /* partial results: (2 per workgroup) x rows x HD, and (M, l) of each row */
     float2 *pml;
-    int *ctr, *stat;
+    int *ctr, *stat;        /* ctr: PG_MANY_WGS x 3, all zero between calls */
 };
 /* The kernel's arguments read again where they are used: held in scalar registers over the loop,
    the ones that only the end needs would be spilled. */

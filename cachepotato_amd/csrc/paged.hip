@@ -252,7 +252,7 @@ extern "C" cpg_paged_ws *cpg_paged_ws_create(int H, int KV, int HD) {
     ws->KV = KV;
     ws->HD = HD;
     ws->rows = (size_t)2 * PG_MANY_WGS * PG_MANY_ROWS;     /* k_paged_few needs an eighth */
-    const size_t sz[5] = {ws->rows * HD * 4, ws->rows * 8, (size_t)3 * PG_FEW_WGS * 4, 4, 2048};
+    const size_t sz[5] = {ws->rows * HD * 4, ws->rows * 8, (size_t)3 * PG_MANY_WGS * 4, 4, 2048};
     size_t total = 0;
     for (int i = 0; i < 5; i++) total += cpg_round256(sz[i]);
     uint8_t *p = (uint8_t *)cpg_malloc(total);
@@ -379,11 +379,11 @@ extern "C" int cpg_paged_attn(const cpg_paged_cache *C, const cpg_paged_batch *B
        as many for an f32 one), two or four steps of k_paged_many; more where the units of the
        largest batch there can be would not fit 31 bits. What an item counts for beside its keys,
        us for 0, 1, 2 and 3 units: prompts of 1500-4500, bf16 295, 260, 251, 253; 512 tokens over 3584,
-       f32 132, 129, 135, 135; 16 conversations, f32 22.2, 20.6, 20.6, 21.7; 96 sequences, bf16, one token
-       each 212, 216, 216, 220 */
+       f32 132, 129, 135, 135; one token each, 16 conversations, f32 20.8, 19.0, 17.1; 96 sequences,
+       bf16 202, 207 */
     a.b = pg_batch{B->q_off, B->len, B->S, B->T, C->KV, B->max_pages, log2_of(C->page),
                    window < PG_MAX_LEN ? window : 0, (a.G + a.hpp - 1) / a.hpp, 0,
-                   few && C->type == CPG_T_F32 ? 6 : 7, C->type == CPG_T_F32 ? 1 : few ? 0 : 2};
+                   few && C->type == CPG_T_F32 ? 6 : 7, few ? (C->type == CPG_T_F32 ? 2 : 0) : C->type == CPG_T_F32 ? 1 : 2};
     while ((2 << a.b.tl) * a.hpp <= rows) a.b.tl++;
     /* no more workgroups than units there can be: tiles of the rows, and keys of a full page row */
     const double tiles = (double)(B->T >> a.b.tl) + (B->S < B->T ? B->S : B->T);

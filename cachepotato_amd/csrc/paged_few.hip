@@ -192,18 +192,24 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_paged_few(const pg_a
 #pragma unroll
             for (int i = 0; i < NS; i++) qf[0][i] = row_ok ? qraw[i] : make_uint4(0, 0, 0, 0);
         } else {
-            float top = 0.0f;
+            int ex = 0;
+            if constexpr (CT == CPG_T_F16) {     /* bf16 has fp32's exponents */
+                float top = 0.0f;
 #pragma unroll
-            for (int i = 0; i < QN; i++) {
-                const uint32_t x[4] = {qraw[i].x, qraw[i].y, qraw[i].z, qraw[i].w};
+                for (int i = 0; i < QN; i++) {
+                    const uint32_t x[4] = {qraw[i].x, qraw[i].y, qraw[i].z, qraw[i].w};
 #pragma unroll
-                for (int j = 0; j < 4; j++) top = fmaxf(top, fabsf(__uint_as_float(x[j])));
+                    for (int j = 0; j < 4; j++) top = fmaxf(top, fabsf(__uint_as_float(x[j])));
+                }
+                top = fmaxf(top, __shfl_xor(top, 16));
+                top = fmaxf(top, __shfl_xor(top, 32));
+                /* the row by 2^-ex, its largest element in [0.5, 1), and the scores by 2^ex */
+                ex = top > 0.0f && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) : 0;
+                cs = ldexpf(cs, ex);
             }
-            top = fmaxf(top, __shfl_xor(top, 16));
-            top = fmaxf(top, __shfl_xor(top, 32));
-            /* the row by 2^-ex, its largest element in [0.5, 1), and the scores by 2^ex */
-            const int ex = top > 0.0f && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) : 0;
-            cs = ldexpf(cs, ex);
+            auto scaled = [&](uint32_t x) {
+                return CT == CPG_T_F16 ? ldexpf(__uint_as_float(x), -ex) : __uint_as_float(x);
+            };
 #pragma unroll
             for (int i = 0; i < NS; i++) {
                 const uint4 r0 = qraw[2 * i], r1 = qraw[2 * i + 1];
@@ -211,8 +217,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_paged_few(const pg_a
                 uint32_t wd[4][NP];
 #pragma unroll
                 for (int j = 0; j < 4; j++)
-                    pg_pieces2<CT, NP>(ldexpf(__uint_as_float(x[2 * j]), -ex),
-                                       ldexpf(__uint_as_float(x[2 * j + 1]), -ex), wd[j]);
+                    pg_pieces2<CT, NP>(scaled(x[2 * j]), scaled(x[2 * j + 1]), wd[j]);
 #pragma unroll
                 for (int n = 0; n < NP; n++)
                     qf[n][i] = row_ok ? make_uint4(wd[0][n], wd[1][n], wd[2][n], wd[3][n]) : make_uint4(0, 0, 0, 0);
