@@ -19,6 +19,7 @@ EXPERTS_AUTO, EXPERTS_GEMV, EXPERTS_MFMA = 0, 1, 2
 ATTN_PER_HEAD, ATTN_SPLIT = 0, 1
 T_F32, T_F16, T_BF16 = 0, 1, 2
 ROPE_HALVES, ROPE_ADJACENT = 0, 1
+PAGED_AUTO, PAGED_FEW, PAGED_MANY = 0, 1, 2
 KT_ROUTE, KT_SELECT, KT_GATEUP, KT_DOWN, KT_COMBINE, KT_FUSED, KT_COUNT = 0, 1, 2, 3, 4, 5, 6
 KT_NAMES = ("route", "select", "gateup", "down", "combine", "fused")
 BLOCK_BYTES = {ENC_Q4: 18, ENC_Q8: 34}
@@ -108,6 +109,7 @@ SIGNATURES = [
     ("cpg_paged_ws_destroy", None, [_vp]),
     ("cpg_paged_ws_status", _i, [_vp]),
     ("cpg_paged_append", _i, [_vp, _vp, _vp, _i, _i, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp]),
+    ("cpg_paged_attn_mode", _i, [_i]),
     ("cpg_paged_attn", _i, [_vp, _vp, _i, _i, _vp, _i64, _f, _i, _vp, _i64, _vp, _vp]),
 ]
 

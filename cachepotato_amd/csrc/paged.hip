@@ -240,6 +240,21 @@ static int log2_of(int x) {
     return l;
 }
 
+/* tiles of `rows` query rows of a kv head: query heads of a row's token, parts that a kv head's make,
+   tokens, and the most tiles that the batch can have (of each part) */
+struct pg_tiling {
+    int hpp, parts, log2_tokens;
+    double tiles;
+};
+
+static pg_tiling tiling(const cpg_paged_batch *B, int G, int rows) {
+    pg_tiling t = {G < rows ? G : rows, 0, 0, 0.0};
+    t.parts = (G + t.hpp - 1) / t.hpp;
+    while ((2 << t.log2_tokens) * t.hpp <= rows) t.log2_tokens++;
+    t.tiles = (double)(B->T >> t.log2_tokens) + (B->S < B->T ? B->S : B->T);
+    return t;
+}
+
 extern "C" cpg_paged_ws *cpg_paged_ws_create(int H, int KV, int HD) {
     if (!g_cpg.ready) { cpg_set_error("cpg_init has not been called"); return nullptr; }
     if (H <= 0 || KV <= 0 || H % KV || !head_dim_ok(HD) || H > 65536) {
@@ -343,6 +358,17 @@ extern "C" int cpg_paged_append(const cpg_paged_cache *C, const cpg_paged_batch 
     return 0;
 }
 
+static int g_paged_mode = CPG_PAGED_AUTO;
+
+extern "C" int cpg_paged_attn_mode(int mode) {
+    if (mode != CPG_PAGED_AUTO && mode != CPG_PAGED_FEW && mode != CPG_PAGED_MANY) {
+        cpg_set_error("cpg_paged_attn_mode: unknown mode %d", mode);
+        return -1;
+    }
+    g_paged_mode = mode;
+    return 0;
+}
+
 extern "C" int cpg_paged_attn(const cpg_paged_cache *C, const cpg_paged_batch *B, int type, int H,
                               const void *q, int64_t ldq, float scale, int window, void *out,
                               int64_t ldo, float *lse, cpg_paged_ws *ws) {
@@ -371,9 +397,20 @@ extern "C" int cpg_paged_attn(const cpg_paged_cache *C, const cpg_paged_batch *B
     a.scale2 = (scale > 0.0f ? scale : 1.0f / sqrtf((float)C->HD)) * 1.4426950408889634f;
     a.blank = ws->blank;
     a.pacc = ws->pacc; a.pml = ws->pml; a.ctr = ws->ctr; a.stat = ws->stat;
-    const bool few = (int64_t)B->max_new * a.G <= PG_FEW_ROWS;
+    /* k_paged_few reads a sequence's keys again for each 16 query rows of a kv head, k_paged_many for
+       each 128: it is ahead where that is the same, and where the items (tiles of 16 rows) are so
+       few that the time is the length of the launch. us, few and many: f32, 32 heads on 4, one
+       sequence over 3000, 44 items 28.6 and 31.4, 96 items 44.4 and 43.2; 8 over 700, 64 items 20.8 and
+       22.9, 128 items 25.7 and 24.1; bf16, 32 heads on 8, 8 over 3000, 128 items 27.8 and 32.2, 384
+       items 60.7 and 37.4. (One sequence over 12000, f32, 44 items 66.3 and 53.9.) */
+    const pg_tiling t16 = tiling(B, a.G, PG_FEW_ROWS);
+    const bool few = g_paged_mode != CPG_PAGED_AUTO
+                         ? g_paged_mode == CPG_PAGED_FEW
+                         : (int64_t)B->max_new * a.G <= PG_FEW_ROWS ||
+                               t16.tiles * C->KV * t16.parts <= (C->type == CPG_T_F32 ? 64 : 128);
     const int rows = few ? PG_FEW_ROWS : PG_MANY_ROWS;
-    a.hpp = a.G < rows ? a.G : rows;
+    const pg_tiling tl = few ? t16 : tiling(B, a.G, rows);
+    a.hpp = tl.hpp;
     a.hinv = (65536 + a.hpp - 1) / a.hpp;
     /* a unit is 128 keys: one step of the four wavefronts of k_paged_few for a 16-bit cache (half
        as many for an f32 one), two or four steps of k_paged_many; more where the units of the
@@ -382,14 +419,12 @@ extern "C" int cpg_paged_attn(const cpg_paged_cache *C, const cpg_paged_batch *B
        f32 132, 129, 135, 135; one token each, 16 conversations, f32 20.8, 19.0, 17.1; 96 sequences,
        bf16 202, 207 */
     a.b = pg_batch{B->q_off, B->len, B->S, B->T, C->KV, B->max_pages, log2_of(C->page),
-                   window < PG_MAX_LEN ? window : 0, (a.G + a.hpp - 1) / a.hpp, 0,
+                   window < PG_MAX_LEN ? window : 0, tl.parts, tl.log2_tokens,
                    few && C->type == CPG_T_F32 ? 6 : 7, few ? (C->type == CPG_T_F32 ? 2 : 0) : C->type == CPG_T_F32 ? 1 : 2};
-    while ((2 << a.b.tl) * a.hpp <= rows) a.b.tl++;
     /* no more workgroups than units there can be: tiles of the rows, and keys of a full page row */
-    const double tiles = (double)(B->T >> a.b.tl) + (B->S < B->T ? B->S : B->T);
     double units;
     for (;; a.b.ul++) {
-        units = tiles * C->KV * a.b.parts * (a.b.extra + ceil(ldexp((double)B->max_pages, a.b.plog - a.b.ul)));
+        units = tl.tiles * C->KV * a.b.parts * (a.b.extra + ceil(ldexp((double)B->max_pages, a.b.plog - a.b.ul)));
         if (units < 2147483648.0 || a.b.ul >= 30) break;
     }
     if (units >= 2147483648.0) {

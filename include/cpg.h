@@ -393,14 +393,23 @@ int cpg_paged_append(const cpg_paged_cache *C, const cpg_paged_batch *B, const c
    out + t * ldo in `type`, and where lse is not NULL lse[t * H + h] = ln sum exp(s_j). A row with no
    key to see gets zeros and lse -infinity. Keys and values that a row does not see do not reach
    it, whatever they hold. Sums, softmax and accumulation are fp32; scores and weights are products
-   of f16 or bf16 matrix instructions: f32 activations in pieces that keep 22 or more bits of
-   them (from about 16 query rows per kv head on, an f32 cache too: keys and values beyond about
-   64000 become infinite there), 16-bit activations with the weights rounded to 16 bits. The way the
+   of matrix instructions, of f32 over an f32 cache, of f16 or bf16 over a 16-bit one: f32
+   activations in pieces that keep 22 or more bits of them, 16-bit activations with the weights
+   rounded to 16 bits. (k_paged_many takes an f32 cache as pairs of f16: keys and values beyond
+   65504 become infinite there.) The way the
    sums are split depends on the batch, and with it the last bits; the same call gives the same
    bits. Asynchronous. */
 int cpg_paged_attn(const cpg_paged_cache *C, const cpg_paged_batch *B, int type, int H,
                    const void *q, int64_t ldq, float scale, int window, void *out, int64_t ldo,
                    float *lse, cpg_paged_ws *ws);
+
+/* The kernel of cpg_paged_attn. CPG_PAGED_AUTO (default): k_paged_few where no sequence has more
+   than 16 query rows per kv head (by max_new) or the batch is small, else k_paged_many.
+   CPG_PAGED_FEW / CPG_PAGED_MANY: always the one (for testing and measuring). */
+#define CPG_PAGED_AUTO 0
+#define CPG_PAGED_FEW  1
+#define CPG_PAGED_MANY 2
+int cpg_paged_attn_mode(int mode);
 
 /* ---------------------------------------------------------------- model glue
  * engine/api/cachepotato.c:108-166, :355-356 */

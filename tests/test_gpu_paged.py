@@ -21,6 +21,16 @@ pytestmark = pytest.mark.gpu
 COMBOS = [(F32, F32), (F32, F16), (F32, BF16), (F16, F16), (BF16, BF16)]
 
 
+@pytest.fixture(autouse=True, params=[C.PAGED_AUTO, C.PAGED_FEW, C.PAGED_MANY], ids=["auto", "few", "many"])
+def mode(request):
+    """every test with the kernel that the batch chooses, and with each of the two"""
+    if request.param != C.PAGED_AUTO and "append" in request.node.name:
+        pytest.skip("no attention")
+    C.check(C.lib().cpg_paged_attn_mode(request.param))
+    yield request.param
+    C.check(C.lib().cpg_paged_attn_mode(C.PAGED_AUTO))
+
+
 def say(*a):
     print(*a, flush=True)
 

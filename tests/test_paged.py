@@ -128,6 +128,13 @@ def test_null_and_workspace_refusals():
     L.cpg_paged_ws_destroy(None)
 
 
+def test_mode_refusals():
+    for mode in (-1, 3):
+        refuse(C.lib().cpg_paged_attn_mode(mode), "mode")
+    for mode in (C.PAGED_FEW, C.PAGED_MANY, C.PAGED_AUTO):
+        assert C.lib().cpg_paged_attn_mode(mode) == 0
+
+
 def test_no_gpu_no_call():
     """right arguments without a context: -7, as from the library's other calls"""
     if C.lib().cpg_current_device() >= 0:
