@@ -148,6 +148,17 @@ __device__ static inline void pg_st_agent16(void *base, uint32_t off, float4 v) 
         v4i_t{__float_as_int(v.x), __float_as_int(v.y), __float_as_int(v.z), __float_as_int(v.w)}, r, off, 0, 16);
 }
 
+/* eight consecutive values to p[i..], a store of 16 bytes for 16-bit types */
+template <int TYPE> __device__ static inline void pg_put8(void *p, size_t i, const float (&x)[8]) {
+    if constexpr (TYPE == CPG_T_F32) {
+        pg_put4<TYPE>(p, i, make_float4(x[0], x[1], x[2], x[3]));
+        pg_put4<TYPE>(p, i + 4, make_float4(x[4], x[5], x[6], x[7]));
+    } else {
+        *(uint4 *)((uint16_t *)p + i) = make_uint4(pg_pack2<TYPE>(x[0], x[1]), pg_pack2<TYPE>(x[2], x[3]),
+                                                   pg_pack2<TYPE>(x[4], x[5]), pg_pack2<TYPE>(x[6], x[7]));
+    }
+}
+
 /* ---------------------------------------------------------------- shares */
 
 /* Where a share begins: the sequence of its first unit and the units before it there. Each

@@ -8,6 +8,13 @@
 
 /* ---------------------------------------------------------------- append */
 
+/* k_paged_append: heads a lane, from APPEND_NI_ROWS rows on (below, one: a launch of few rows is
+   shorter with more workgroups). us for 1, 2, 3 and 4: prompts of 9 k rows, 32 heads on 8, bf16
+   57.0, 53.6, 48.7 (4.8 TB/s in and out, a copy's rate), 49.2; 512 rows, 32 on 4, f32 7.9, 8.4, 8.9,
+   9.3 */
+#define APPEND_NI 3
+#define APPEND_NI_ROWS 2048
+
 struct pg_append {
     const void *q, *k, *v;
     void *q_out, *kc, *vc;
@@ -36,23 +43,32 @@ __device__ static inline int pg_row_seq(const int *__restrict__ q_off, int S, in
 }
 
 /* grid (T, parts of the H + 2 KV heads), 256 threads: row t, 2^gl lanes to a head, eight elements a
-   lane (HD = 96 and 192 leave a quarter of the lanes idle). A query or key head is normed (its sum
-   of squares over the lanes in fp32), turned, and rounded once where it is stored; a value head is
-   only stored. The partner of a lane's elements in the rotation is a lane's whole eight, since rot
-   is a multiple of 16: rot / 16 lanes away, or its own.
-   Bound by the bytes of the heads in and out; for a few rows by the chain of launch, row's
-   sequence, page id, store. */
-template <int AT, int CT>
+   lane (HD = 96 and 192 leave a quarter of the lanes idle), NI heads a lane, 256 >> gl apart. A query or
+   key head is normed (its sum of squares over the lanes in fp32), turned, and rounded once where it
+   is stored; a value head is only stored. The partner of a lane's elements in the rotation is a
+   lane's whole eight, since rot is a multiple of 16: rot / 16 lanes away, or its own. A lane's place in
+   its heads is the same, so the row's search, page and rotation pairs serve all of them.
+   Bound by the bytes of the heads in and out (APPEND_NI); for a few rows by the chain of launch,
+   row's sequence, page id, store: 3.3 us for one row. */
+template <int AT, int CT, int NI>
 __global__ __launch_bounds__(256) void k_paged_append(const pg_append a, int gl) {
-    const int t = blockIdx.x, tid = threadIdx.x, li = tid & ((1 << gl) - 1);
-    const int head = (blockIdx.y * 256 + tid) >> gl, heads = a.H + 2 * a.KV;
-    const bool live = head < heads && li * 8 < a.HD;
-    const int hc = min(head, heads - 1), lc = min(li, a.HD / 8 - 1);
-    const bool isq = hc < a.H, isv = hc >= a.H + a.KV;
-    const int hh = isq ? hc : isv ? hc - a.H - a.KV : hc - a.H;
+    const int t = blockIdx.x, tid = threadIdx.x, li = tid & ((1 << gl) - 1), hpw = 256 >> gl;
+    const int head0 = blockIdx.y * NI * hpw + (tid >> gl), heads = a.H + 2 * a.KV;
+    const bool in = li * 8 < a.HD;
+    const int lc = min(li, a.HD / 8 - 1);
     typedef typename pg_elem<AT>::t at;
-    const at *src = (const at *)(isq ? a.q : isv ? a.v : a.k) +
-                    (size_t)t * (isq ? a.ldq : isv ? a.ldv : a.ldk) + (size_t)hh * a.HD + 8 * lc;
+    constexpr int NR = AT == CPG_T_F32 ? 2 : 1;
+    uint4 raw[NI][NR];
+#pragma unroll
+    for (int i = 0; i < NI; i++) {               /* unconditional, a head past the last the last */
+        const int hc = min(head0 + i * hpw, heads - 1);
+        const bool isq = hc < a.H, isv = hc >= a.H + a.KV;
+        const int hh = isq ? hc : isv ? hc - a.H - a.KV : hc - a.H;
+        const at *src = (const at *)(isq ? a.q : isv ? a.v : a.k) +
+                        (size_t)t * (isq ? a.ldq : isv ? a.ldv : a.ldk) + (size_t)hh * a.HD + 8 * lc;
+#pragma unroll
+        for (int j = 0; j < NR; j++) raw[i][j] = ((const uint4 *)src)[j];
+    }
     const int s = pg_row_seq(a.q_off, a.S, t);
     if (s < 0) return;
     const pg_seq sq = pg_get_seq(a.q_off, a.len, s, a.T, a.max_pages, a.plog);
@@ -66,83 +82,85 @@ __global__ __launch_bounds__(256) void k_paged_append(const pg_append a, int gl)
     const int page = bad ? -1 : a.pages[(size_t)s * a.max_pages + (pc >> a.plog)];
     const bool miss = page < 0 || page >= a.n_pages;
     if (miss && tid == 0) *a.stat = 1;
-    float x[8];
-    if constexpr (AT == CPG_T_F32) {
-        const float4 u = ((const float4 *)src)[0], w = ((const float4 *)src)[1];
-        x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
-        x[4] = w.x; x[5] = w.y; x[6] = w.z; x[7] = w.w;
-    } else {
-        const uint4 u = *(const uint4 *)src;
-        const uint32_t uw[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const float2 f = pg_unpack2<AT>(uw[i]);
-            x[2 * i] = f.x;
-            x[2 * i + 1] = f.y;
-        }
-    }
-    const float *gain = isq ? a.q_norm : a.k_norm;
-    if (gain && !isv) {
-        float ss = 0.0f;
-        if (li * 8 < a.HD)
-#pragma unroll
-            for (int i = 0; i < 8; i++) ss = fmaf(x[i], x[i], ss);
-        for (int o = 1; o < 1 << gl; o <<= 1) ss += __shfl_xor(ss, o);
-        const float inv = __fdiv_rn(1.0f, cpg_sqrt_rn(__fadd_rn(__fdiv_rn(ss, (float)a.HD), a.eps)));
-        const float4 g0 = ((const float4 *)gain)[2 * lc], g1 = ((const float4 *)gain)[2 * lc + 1];
-        const float g[8] = {g0.x, g0.y, g0.z, g0.w, g1.x, g1.y, g1.z, g1.w};
-#pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = __fmul_rn(__fmul_rn(x[i], inv), g[i]);
-    }
-    if (a.rot > 0) {                             /* shuffles: every lane takes part */
-        const bool turn = !isv && 8 * li < a.rot;
+    /* the lane's rotation: pairs of its elements and of another lane's (halves), or among its own */
+    const bool turn = 8 * li < a.rot;
+    const int hl = a.rot / 16;                   /* lanes of half the rotated elements */
+    const bool upper = li >= hl;
+    const int lane = tid & 63, other = turn ? (upper ? lane - hl : lane + hl) : lane;
+    float cs[8], sn[8];
+    if (a.rot > 0) {
         const float4 *row = (const float4 *)(a.table + (size_t)pc * a.rot);
-        if (a.adjacent) {
-            const int c = turn ? 2 * li : 0;     /* pairs 4 li .. 4 li + 3, two to a float4 */
-            const float4 r0 = row[c], r1 = row[c + 1];
-            const float cs[8] = {r0.x, r0.y, r0.z, r0.w, r1.x, r1.y, r1.z, r1.w};
-            if (turn)
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float u = x[2 * i], w = x[2 * i + 1], cc = cs[2 * i], sn = cs[2 * i + 1];
-                    x[2 * i] = __fsub_rn(__fmul_rn(u, cc), __fmul_rn(w, sn));
-                    x[2 * i + 1] = __fadd_rn(__fmul_rn(w, cc), __fmul_rn(u, sn));
-                }
-        } else {
-            const int hl = a.rot / 16;           /* lanes of half the rotated elements */
-            const bool upper = li >= hl;
-            const int c = turn ? 4 * (upper ? li - hl : li) : 0;
-            const int lane = tid & 63, other = turn ? (upper ? lane - hl : lane + hl) : lane;
-            float cs[16];
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float4 r = row[c + i];
-                cs[4 * i] = r.x; cs[4 * i + 1] = r.y; cs[4 * i + 2] = r.z; cs[4 * i + 3] = r.w;
-            }
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const float y = __shfl(x[i], other), cc = cs[2 * i], sn = cs[2 * i + 1];
-                const float down = __fsub_rn(__fmul_rn(x[i], cc), __fmul_rn(y, sn));
-                const float up = __fadd_rn(__fmul_rn(x[i], cc), __fmul_rn(y, sn));
-                x[i] = turn ? (upper ? up : down) : x[i];
-            }
+        for (int i = 0; i < 4; i++) {            /* two pairs to a float4 */
+            const float4 r = row[a.adjacent ? (turn ? 2 * li + (i >> 1) : 0)
+                                            : (turn ? 4 * (upper ? li - hl : li) : 0) + i];
+            cs[2 * i] = r.x; sn[2 * i] = r.y; cs[2 * i + 1] = r.z; sn[2 * i + 1] = r.w;
         }
     }
-    if (!live) return;
-    if (isq) {
-        if (bad)
 #pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = __int_as_float(0x7fc00000);
-        const size_t e = (size_t)t * a.ldqo + (size_t)hh * a.HD + 8 * li;
-        pg_put4<AT>(a.q_out, e, make_float4(x[0], x[1], x[2], x[3]));
-        pg_put4<AT>(a.q_out, e + 4, make_float4(x[4], x[5], x[6], x[7]));
-    } else if (!miss) {
-        const size_t e = (size_t)page * a.page_stride +
-                         (size_t)(pos & ((1 << a.plog) - 1)) * a.slot_stride +
-                         (size_t)hh * a.head_stride + 8 * li;
-        void *dst = isv ? a.vc : a.kc;
-        pg_put4<CT>(dst, e, make_float4(x[0], x[1], x[2], x[3]));
-        pg_put4<CT>(dst, e + 4, make_float4(x[4], x[5], x[6], x[7]));
+    for (int i = 0; i < NI; i++) {
+        const int head = head0 + i * hpw, hc = min(head, heads - 1);
+        const bool isq = hc < a.H, isv = hc >= a.H + a.KV;
+        const int hh = isq ? hc : isv ? hc - a.H - a.KV : hc - a.H;
+        float x[8];
+        if constexpr (AT == CPG_T_F32) {
+            const uint32_t w[8] = {raw[i][0].x, raw[i][0].y, raw[i][0].z, raw[i][0].w,
+                                   raw[i][NR - 1].x, raw[i][NR - 1].y, raw[i][NR - 1].z, raw[i][NR - 1].w};
+#pragma unroll
+            for (int j = 0; j < 8; j++) x[j] = __uint_as_float(w[j]);
+        } else {
+            const uint32_t w[4] = {raw[i][0].x, raw[i][0].y, raw[i][0].z, raw[i][0].w};
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float2 f = pg_unpack2<AT>(w[j]);
+                x[2 * j] = f.x;
+                x[2 * j + 1] = f.y;
+            }
+        }
+        const float *gain = isq ? a.q_norm : a.k_norm;
+        if (a.q_norm || a.k_norm) {              /* shuffles: every lane takes part */
+            float ss = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; j++) ss = fmaf(x[j], x[j], ss);
+            ss = in ? ss : 0.0f;
+            for (int o = 1; o < 1 << gl; o <<= 1) ss += __shfl_xor(ss, o);
+            if (gain && !isv) {
+                const float inv = __fdiv_rn(1.0f, cpg_sqrt_rn(__fadd_rn(__fdiv_rn(ss, (float)a.HD), a.eps)));
+                const float4 g0 = ((const float4 *)gain)[2 * lc], g1 = ((const float4 *)gain)[2 * lc + 1];
+                const float g[8] = {g0.x, g0.y, g0.z, g0.w, g1.x, g1.y, g1.z, g1.w};
+#pragma unroll
+                for (int j = 0; j < 8; j++) x[j] = __fmul_rn(__fmul_rn(x[j], inv), g[j]);
+            }
+        }
+        if (a.rot > 0 && a.adjacent) {
+            if (turn && !isv)
+#pragma unroll
+                for (int j = 0; j < 4; j++) {    /* pair j of the lane: read as pairs 2 (j / 2) + j % 2 */
+                    const int c = 4 * (j >> 1) + (j & 1);
+                    const float u = x[2 * j], w = x[2 * j + 1];
+                    x[2 * j] = __fsub_rn(__fmul_rn(u, cs[c]), __fmul_rn(w, sn[c]));
+                    x[2 * j + 1] = __fadd_rn(__fmul_rn(w, cs[c]), __fmul_rn(u, sn[c]));
+                }
+        } else if (a.rot > 0) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const float y = __shfl(x[j], other);
+                const float down = __fsub_rn(__fmul_rn(x[j], cs[j]), __fmul_rn(y, sn[j]));
+                const float up = __fadd_rn(__fmul_rn(x[j], cs[j]), __fmul_rn(y, sn[j]));
+                x[j] = turn && !isv ? (upper ? up : down) : x[j];
+            }
+        }
+        if (!in || head >= heads) continue;
+        if (isq) {
+            if (bad)
+#pragma unroll
+                for (int j = 0; j < 8; j++) x[j] = __int_as_float(0x7fc00000);
+            pg_put8<AT>(a.q_out, (size_t)t * a.ldqo + (size_t)hh * a.HD + 8 * li, x);
+        } else if (!miss) {
+            pg_put8<CT>(isv ? a.vc : a.kc,
+                        (size_t)page * a.page_stride + (size_t)(pos & ((1 << a.plog) - 1)) * a.slot_stride +
+                            (size_t)hh * a.head_stride + 8 * li, x);
+        }
     }
 }
 
@@ -303,6 +321,19 @@ extern "C" int cpg_paged_ws_status(cpg_paged_ws *ws) {
     return v;
 }
 
+template <int NI> static int launch_append(const pg_append &a, int type, int cache) {
+    const int gl = log2_of(a.HD / 8), hpw = (256 >> gl) * NI;
+    const dim3 grid(a.T, (a.H + 2 * a.KV + hpw - 1) / hpw);
+    auto kernel = type == CPG_T_F16    ? k_paged_append<CPG_T_F16, CPG_T_F16, NI>
+                  : type == CPG_T_BF16 ? k_paged_append<CPG_T_BF16, CPG_T_BF16, NI>
+                  : cache == CPG_T_F32 ? k_paged_append<CPG_T_F32, CPG_T_F32, NI>
+                  : cache == CPG_T_F16 ? k_paged_append<CPG_T_F32, CPG_T_F16, NI>
+                                       : k_paged_append<CPG_T_F32, CPG_T_BF16, NI>;
+    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, g_cpg.stream, a, gl);
+    CPG_LAUNCH_CHECK("k_paged_append");
+    return 0;
+}
+
 extern "C" int cpg_paged_append(const cpg_paged_cache *C, const cpg_paged_batch *B,
                                 const cpg_paged_rope *R, int type, int H, const void *q, int64_t ldq,
                                 const void *k, int64_t ldk, const void *v, int64_t ldv, void *q_out,
@@ -346,16 +377,7 @@ extern "C" int cpg_paged_append(const cpg_paged_cache *C, const cpg_paged_batch 
     a.H = H; a.KV = C->KV; a.HD = C->HD; a.S = B->S; a.T = B->T;
     a.max_pages = B->max_pages; a.n_pages = C->n_pages; a.plog = log2_of(C->page);
     a.stat = ws->stat;
-    const int gl = log2_of(C->HD / 8), hpw = 256 >> gl;
-    const dim3 grid(B->T, (H + 2 * C->KV + hpw - 1) / hpw);
-    auto kernel = type == CPG_T_F16    ? k_paged_append<CPG_T_F16, CPG_T_F16>
-                  : type == CPG_T_BF16 ? k_paged_append<CPG_T_BF16, CPG_T_BF16>
-                  : C->type == CPG_T_F32 ? k_paged_append<CPG_T_F32, CPG_T_F32>
-                  : C->type == CPG_T_F16 ? k_paged_append<CPG_T_F32, CPG_T_F16>
-                                         : k_paged_append<CPG_T_F32, CPG_T_BF16>;
-    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, g_cpg.stream, a, gl);
-    CPG_LAUNCH_CHECK("k_paged_append");
-    return 0;
+    return B->T < APPEND_NI_ROWS ? launch_append<1>(a, type, C->type) : launch_append<APPEND_NI>(a, type, C->type);
 }
 
 static int g_paged_mode = CPG_PAGED_AUTO;
