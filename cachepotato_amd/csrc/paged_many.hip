@@ -510,7 +510,10 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_paged_many(const pg_
             if (tid == 0) wild_s[turn & 3] = 0;  /* noted again four steps on, with barriers between */
             turn++;
         }
-        if (steps == 0) turn++;
+        if (steps == 0) {                        /* the step that was staged for nothing */
+            if (tid == 0) wild_s[turn & 3] = 0;
+            turn++;
+        }
         l = pg_half_sum(l);
 
         /* ---- the rows: written, or left as a piece. A lane's elements 8 e + 4 h .. + 3 of its row */
