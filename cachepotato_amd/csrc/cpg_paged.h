@@ -165,7 +165,9 @@ template <int TYPE> __device__ static inline void pg_put8(void *p, size_t i, con
    wavefront finds it by itself, without a barrier: lane l counts the units of sequences l c .. l c +
    c - 1 (c = S / 64, rounded up), a scan over the lanes gives all units and the lane whose sequences
    hold the first of the share, and those are gone through in the same way. stat: the workspace's
-   status word, set where the batch cannot be followed. */
+   status word, set where the batch cannot be followed. Rows that do not ascend within 0 .. T are no
+   batch (two sequences could have a row, and the units would pass their bound): then there is no
+   share, in no workgroup, since each looks at all of them. */
 struct pg_start {
     int s;
     uint32_t rem;
@@ -183,14 +185,17 @@ __device__ static inline uint32_t pg_wave_scan(uint32_t v) {         /* inclusiv
 
 __device__ static inline pg_share pg_find_share(const pg_batch &b, pg_start &st, int *stat) {
     const int lane = threadIdx.x & 63;
+    bool cut = false;
     auto units = [&](int s) {
         const pg_seq q = pg_get_seq(b.q_off, b.len, s, b.T, b.max_pages, b.plog);
         if (blockIdx.x == 0 && q.bad && (q.cut || q.n > 0)) *stat = 1;
+        cut |= q.cut;
         return pg_seq_units(b, q);
     };
     st.s = 0;
     if (b.S == 1) {
-        const pg_share r = pg_deal(units(0), blockIdx.x, gridDim.x);
+        const uint32_t U = units(0);
+        const pg_share r = pg_deal(cut ? 0 : U, blockIdx.x, gridDim.x);
         st.rem = r.u0;
         return r;
     }
@@ -201,7 +206,7 @@ __device__ static inline pg_share pg_find_share(const pg_batch &b, pg_start &st,
         mine += s < n ? units(s) : 0;
     }
     uint32_t inc = pg_wave_scan(mine);
-    const pg_share r = pg_deal(__builtin_amdgcn_readlane(inc, 63), blockIdx.x, gridDim.x);
+    const pg_share r = pg_deal(__any(cut) ? 0 : __builtin_amdgcn_readlane(inc, 63), blockIdx.x, gridDim.x);
     st.rem = r.u0;
     if (r.u0 == r.u1) return r;
     for (;;) {

@@ -338,10 +338,10 @@ typedef struct {
    q_off[s+1] - 1 are sequence s's (q_off ascending, within 0 .. T; none is allowed), in the order
    of their positions, which end at len[s] - 1: len[s] counts the tokens in the cache with the new
    ones. Its token j lies in slot j % page of page pages[s * max_pages + j / page]. Rows that no
-   sequence has (behind q_off[S], as in a padded batch) are neither read nor written. The three
+   sequence has (behind q_off[S], as in a padded batch) are not written. The three
    arrays are read on the device when the kernels run, so a captured graph can be replayed as the
-   batch moves on. T and each len are at most 2^30. max_new: about how many new tokens the longest sequence brings; it chooses
-   between kernels for few and for many tokens and is not relied on. */
+   batch moves on. T and each len are at most 2^30. max_new: about how many new tokens the longest
+   sequence brings; it chooses between kernels for few and for many tokens and is not relied on. */
 typedef struct {
     int S, T, max_new, max_pages;
     const int *pages, *q_off, *len;     /* device: (S, max_pages), (S + 1), (S) */
@@ -361,19 +361,20 @@ typedef struct {
     float eps;
 } cpg_paged_rope;
 
-/* Scratch for layers of H query heads, KV key/value heads and head_dim HD; one call at a time
-   per workspace (calls in stream order, and graphs replayed on the stream, are). */
+/* Scratch (512 KiB per element of head_dim: 67 MB at 128) for layers of H query heads, KV key/value
+   heads and head_dim HD; one call at a time per workspace (calls in stream order, and graphs
+   replayed on the stream, are). */
 typedef struct cpg_paged_ws cpg_paged_ws;
 cpg_paged_ws *cpg_paged_ws_create(int H, int KV, int HD);
 void cpg_paged_ws_destroy(cpg_paged_ws *ws);
 /* Synchronises, then returns 1 when a call on ws since the last cpg_paged_ws_status met batch
    data that it could not follow (and clears that), 0 when none did, negative on a device error.
-   Nothing outside the pool is touched for such data: q_off is taken within 0 .. T and ascending;
-   a sequence whose len is negative, beyond max_pages * page or beyond 2^30, a row whose position is negative or
-   beyond the rotation table, or a page id outside [0, n_pages) leaves the pool as it was, and
-   query rows of cpg_paged_append (not for a page id) and rows of cpg_paged_attn that depend on it
-   become NaN. (In cpg_paged_attn a row at a negative position has no key to see: zeros, not an
-   error.) */
+   Nothing outside the pool is touched for such data. A q_off that does not ascend within 0 .. T:
+   cpg_paged_attn writes nothing, cpg_paged_append goes by what lies within. A sequence whose len is
+   negative, beyond max_pages * page or beyond 2^30, a row whose position is negative or beyond the
+   rotation table, or a page id outside [0, n_pages) leaves the pool as it was, and query rows of
+   cpg_paged_append (not for a page id) and rows of cpg_paged_attn that depend on it become NaN. (In
+   cpg_paged_attn a row at a negative position has no key to see: zeros, not an error.) */
 int cpg_paged_ws_status(cpg_paged_ws *ws);
 
 /* Row t's query heads q + t * ldq (H of HD), key heads k + t * ldk and value heads v + t * ldv (KV
@@ -396,9 +397,8 @@ int cpg_paged_append(const cpg_paged_cache *C, const cpg_paged_batch *B, const c
    of matrix instructions, of f32 over an f32 cache, of f16 or bf16 over a 16-bit one: f32
    activations in pieces that keep 22 or more bits of them, 16-bit activations with the weights
    rounded to 16 bits. (k_paged_many takes an f32 cache as pairs of f16: keys and values beyond
-   65504 become infinite there.) The way the
-   sums are split depends on the batch, and with it the last bits; the same call gives the same
-   bits. Asynchronous. */
+   65504 become infinite there.) The way the sums are split depends on the batch, and with it the
+   last bits; the same call gives the same bits. out may not overlap q. Asynchronous. */
 int cpg_paged_attn(const cpg_paged_cache *C, const cpg_paged_batch *B, int type, int H,
                    const void *q, int64_t ldq, float scale, int window, void *out, int64_t ldo,
                    float *lse, cpg_paged_ws *ws);

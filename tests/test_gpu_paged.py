@@ -121,6 +121,27 @@ def test_window(cpg, window, type_, ctype):
     run([(300, 1), (90, 90), (260, 30), (3, 3)], 4, 2, 64, 16, type_, ctype, window=window)
 
 
+@pytest.mark.parametrize("window", [1, 5, 40])
+def test_window_and_rows_without_keys(cpg, window):
+    """sequences shorter than their new rows, under a window"""
+    run([(3, 9), (40, 70), (0, 2), (50, 50), (60, 1)], 8, 2, 64, 16, F32, F32, window=window)
+    run([(3, 9), (40, 70), (0, 2), (50, 50), (60, 1)], 4, 2, 64, 16, BF16, BF16, window=window)
+
+
+def test_rows_that_do_not_ascend(cpg):
+    """offsets that give the same rows to many sequences, whose units would pass every bound: nothing
+    is written, with one sequence, within a wavefront's reach and beyond"""
+    for S in (2, 64, 300):
+        b = Batch([(60, 4)] * S, 1, 64, 16, F32).fill().upload()
+        b.off = np.array([0, b.T] * S, np.int32)[:S + 1]
+        b.upload()
+        ws = Workspace(4, 1, 64)
+        out, lse = attend(b, ws, np.zeros((b.T, 4, 64)), 4, F32)
+        assert ws.status() == 1 and np.isnan(out).all() and np.isnan(lse).all()
+        ws.close()
+        b.close()
+
+
 def test_window_pages_are_not_looked_at(cpg):
     """pages behind every row's window may have been given to others: their ids may be anything"""
     b = Batch([(400, 1), (390, 21)], 2, 64, 16, F32).fill()
@@ -327,6 +348,8 @@ def test_bad_lengths_and_offsets(cpg):
         b.upload()
         attend(b, ws, q, 8, F32)                     # nothing outside the rows is touched
         assert ws.status() == 1
+        out, lse = attend(b, ws, q, 8, F32)          # not a row is written
+        assert ws.status() == 1 and np.isnan(out).all() and np.isnan(lse).all()
     b.off = off
     b.upload()
     out, _ = attend(b, ws, q, 8, F32)
