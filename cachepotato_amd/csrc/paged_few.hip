@@ -478,14 +478,16 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_paged_few(const pg_a
                 const int n = min(MG, wl - gx + 1);
                 mine = last_arriver(&late->ctr[2 * gx + (gx == wf)], n - 1, &flag);
                 if (mine) {
-                    for (int i0 = 0; i0 < rows * (HD / 4); i0 += 256) {
-                        const int i = i0 + te, ic = min(i, rows * (HD / 4) - 1);
+                    /* whole rows a pass: a row's (M, l) is replaced once all of the row has it */
+                    constexpr int PASS = 256 / (HD / 4) * (HD / 4);
+                    for (int i0 = 0; i0 < rows * (HD / 4); i0 += PASS) {
+                        const int end = min(i0 + PASS, rows * (HD / 4)), i = i0 + te, ic = min(i, end - 1);
                         const int r = ic / (HD / 4), d = ic % (HD / 4) * 4;
                         float4 v;
                         float top, L;
                         merge(gx, n, 1, r, d, v, top, L);
                         __syncthreads();         /* every thread of the row has read its (M, l) */
-                        if (i < rows * (HD / 4)) put(place(gx), r, d, v, top, L);
+                        if (i < end) put(place(gx), r, d, v, top, L);
                     }
                 }
             }

@@ -281,6 +281,14 @@ def test_long_context_split(cpg):
     run([(3000, 10), (20, 1), (1, 1), (900, 300)], 4, 2, 64, 16, F32, F32)
 
 
+@pytest.mark.parametrize("type_,ctype", [(F32, F32), (BF16, BF16)])
+@pytest.mark.parametrize("HD", [64, 96, 128, 192, 256])
+def test_item_of_many_pieces(cpg, HD, type_, ctype):
+    """an item over all workgroups, its pieces merged in groups, with all of a tile's rows"""
+    run([(9000, 1)], 16, 1, HD, 64, type_, ctype)
+    run([(7000, 9)], 14, 1, HD, 64, type_, ctype)
+
+
 def test_strided_rows(cpg):
     """q as the head part of a wider row, out into a wider row"""
     b = Batch([(40, 1), (60, 25)], 2, 128, 16, F32).fill().upload()
