@@ -451,45 +451,48 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_paged_many(const pg_
                 }
                 __builtin_amdgcn_s_setprio(0);
                 if (wild) {
-                    /* The rest, for the rows that see it, from the pages again: in memory, in the place
-                       that the item's piece may take when it is done, so that this seldom path
-                       holds no registers */
+                    /* The rest, for the rows that see it (their weights taken as above zero), from the
+                       pages again: in memory, in the place that the item's piece may take when it is
+                       done, so that this seldom path holds no registers */
                     const pg_args *la = pg_late_args();
-                    float4 *mine = (float4 *)((uint8_t *)la->pacc +
-                                              ((size_t)2 * me + (me == pg_owner(it.first, sh.U, W))) * P::SLOT) +
-                                   w * (ND * 256) + lane;
+                    uint8_t *mine = (uint8_t *)la->pacc +
+                                    ((size_t)2 * me + (me == pg_owner(it.first, sh.U, W))) * P::SLOT +
+                                    (size_t)w * (ND * 4096);
+                    /* stored and loaded as pieces are, since another XCD may write there later */
 #pragma unroll
                     for (int i = 0; i < 4 * ND; i++)
-                        mine[64 * i] = make_float4(o[i >> 2][4 * (i & 3)], o[i >> 2][4 * (i & 3) + 1],
-                                                   o[i >> 2][4 * (i & 3) + 2], o[i >> 2][4 * (i & 3) + 3]);
+                        pg_st_agent16(mine, 1024 * i + 16 * lane,
+                                      make_float4(o[i >> 2][4 * (i & 3)], o[i >> 2][4 * (i & 3) + 1],
+                                                  o[i >> 2][4 * (i & 3) + 2], o[i >> 2][4 * (i & 3) + 3]));
+                    mem_done();
 #pragma nounroll
-                    for (int j = max(jb, klo); j < min(jb + KT, khi); j++) {
-                        const uint32_t vid = (uint32_t)ids[j >> a.b.plog];
-                        if (vid >= (uint32_t)a.n_pages) continue;
-                        const uint64_t vp = (uint64_t)vb + ((uint64_t)(vid * a.page_units + (uint32_t)(j & pmask) * a.slot_units) << a.ush);
-                        if (j > pos || j < pos_lo) continue;
+                    for (int i = 0; i < 4 * ND; i++) {
+                        const v4i_t r = ld_agent16(mine, 1024 * i + 16 * lane);
+                        float x[4];
+#pragma unroll
+                        for (int k = 0; k < 4; k++) x[k] = __int_as_float(r[k]);
 #pragma nounroll
-                        for (int i = 0; i < 4 * ND; i++) {
-                            float4 x = mine[64 * i];
-                            float *xs = &x.x;
+                        for (int j = max(jb, klo); j < min(jb + KT, khi); j++) {
+                            const uint32_t vid = (uint32_t)ids[j >> a.b.plog];
+                            if (vid >= (uint32_t)a.n_pages || j > pos || j < pos_lo) continue;
+                            const uint64_t vp = (uint64_t)vb + ((uint64_t)(vid * a.page_units + (uint32_t)(j & pmask) * a.slot_units) << a.ush);
 #pragma unroll
                             for (int k = 0; k < 4; k++) {
                                 const int e = 8 * i + 4 * h + k;
                                 float y;
                                 if constexpr (F32) y = pg_load<float>(vp + 4 * e);
                                 else y = pg_unpack2<CT>(pg_load<uint16_t>(vp + 2 * e)).x;
-                                xs[k] += fabsf(y) < INFINITY ? 0.0f : y;
+                                x[k] += fabsf(y) < INFINITY ? 0.0f : y;
                             }
-                            mine[64 * i] = x;
                         }
+                        pg_st_agent16(mine, 1024 * i + 16 * lane, make_float4(x[0], x[1], x[2], x[3]));
                     }
+                    mem_done();
 #pragma unroll
                     for (int i = 0; i < 4 * ND; i++) {
-                        const float4 x = mine[64 * i];
-                        o[i >> 2][4 * (i & 3)] = x.x;
-                        o[i >> 2][4 * (i & 3) + 1] = x.y;
-                        o[i >> 2][4 * (i & 3) + 2] = x.z;
-                        o[i >> 2][4 * (i & 3) + 3] = x.w;
+                        const v4i_t x = ld_agent16(mine, 1024 * i + 16 * lane);
+#pragma unroll
+                        for (int k = 0; k < 4; k++) o[i >> 2][4 * (i & 3) + k] = __int_as_float(x[k]);
                     }
                     /* waited for here: where the paths join it would be in every step, and for the
                        copies in flight too */
