@@ -52,6 +52,7 @@ template <int CT, int AT, int HD> struct pg_many_t {
     __host__ __device__ static constexpr int kswz(int r) { return CPR == 8 ? (r >> 1) & 7 : r & 15; }
     __host__ __device__ static constexpr int vswz(int r) { return CPR == 8 ? ((r >> 1) & 3) << 1 : (r & 7) << 1; }
 };
+#define PG_NO_SCALE (-300)  /* of values that are all zero: below any other's */
 #define PG_SLACK 8.0f       /* log2 of how far a score may pass the maximum that weights refer to */
 
 template <int OT>
@@ -93,7 +94,8 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_paged_many(const pg_
     constexpr int NQ = P::NQ, NC = P::NC, OT = P::OT, KT = P::KT, RB = P::RB, CPR = P::CPR, NB = P::NB,
                   NS = P::NS, ND = P::ND, E = P::E;
     extern __shared__ __align__(16) uint8_t lds[];       /* two buffers: K planes, V planes each */
-    __shared__ int flag, wild_s[4];          /* wild_s: of a step, by its number among all steps */
+    __shared__ int flag, wild_s[4];          /* wild_s, scale_s: of a step, by its number among all steps */
+    __shared__ __align__(16) int scale_s[4][4];
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     pg_start at;
     const pg_share sh = pg_find_share(a.b, at, a.stat);
@@ -247,12 +249,18 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_paged_many(const pg_
             uint32_t any = 0;
             if constexpr (F32) {
 #pragma unroll
-                for (int e = 0; e < EF; e++)
+                for (int e = 0; e < EF; e++) {
+                    /* what no row sees has no say in the scale either */
+                    const int j = j0 + KT * n + P::RW * w + row_e(e);
+                    const uint32_t seen = j >= klo && j < khi ? ~0u : 0u;
 #pragma unroll
                     for (int i = 0; i < 8; i++) {
+                        kraw[e][i >> 2][i & 3] &= seen;
+                        vraw[e][i >> 2][i & 3] &= seen;
                         any |= pg_wild<CPG_T_F32>(vraw[e][i >> 2][i & 3]);
                         vraw[e][i >> 2][i & 3] = pg_tame<CPG_T_F32>(vraw[e][i >> 2][i & 3]);
                     }
+                }
             } else {
 #pragma unroll
                 for (int e = 0; e < E; e++) {
@@ -265,9 +273,44 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_paged_many(const pg_
             if (__any(any != 0)) wild_s[turn & 3] = 1;
         };
 
+        /* f32 caches: the wavefront's rows by powers of two 2^-ek and 2^-ev that bring their largest key
+           and value element within f16's range and its precision, 2^-3 .. 2^15: where it is within,
+           none. The scores take ek back, and the sums of values ev. */
+        auto scale = [&](int turn) __attribute__((always_inline)) {
+            float tk = 0.0f, tv = 0.0f;
+#pragma unroll
+            for (int e = 0; e < EF; e++)
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    tk = fmaxf(tk, fabsf(__uint_as_float(kraw[e][i >> 2][i & 3])));
+                    tv = fmaxf(tv, fabsf(__uint_as_float(vraw[e][i >> 2][i & 3])));
+                }
+            const bool kin = __any(tk >= 0.125f) && !__any(tk > 32768.0f);
+            const bool vin = __any(tv >= 0.125f) && !__any(tv > 32768.0f);
+            int ek = 0, ev = 0;
+            if (!kin || !vin) {
+#pragma nounroll
+                for (int o = 1; o < 64; o <<= 1) {
+                    tk = fmaxf(tk, __shfl_xor(tk, o));
+                    tv = fmaxf(tv, __shfl_xor(tv, o));
+                }
+                if (!kin && tk > 0.0f && tk < INFINITY) ek = __builtin_amdgcn_frexp_expf(tk) - 8;
+                if (!vin && tv < INFINITY) ev = tv > 0.0f ? __builtin_amdgcn_frexp_expf(tv) - 8 : PG_NO_SCALE;
+#pragma unroll
+                for (int e = 0; e < EF; e++)
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        kraw[e][i >> 2][i & 3] = __float_as_uint(ldexpf(__uint_as_float(kraw[e][i >> 2][i & 3]), -ek));
+                        vraw[e][i >> 2][i & 3] = __float_as_uint(ldexpf(__uint_as_float(vraw[e][i >> 2][i & 3]), -ev));
+                    }
+            }
+            if (lane == 0) scale_s[turn & 3][w] = (ek & 0xFFFF) | (int)((uint32_t)ev << 16);
+        };
+
         f32x16_t o[ND];
 #pragma unroll
         for (int d = 0; d < ND; d++) o[d] = f32x16_t{};
+        int Ev = PG_NO_SCALE;                    /* f32 caches: o counts in 2^Ev */
         float M = -INFINITY, l = 0.0f;           /* what the weights refer to, in log2; -inf: nothing yet */
 
         int id = load_id(0);
@@ -316,6 +359,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_paged_many(const pg_
         }
         if constexpr (F32) {
             note(0, 0, turn);
+            scale(turn);
             store(0);
         } else {
             wait_vm_lgkm<0>();
@@ -369,6 +413,28 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_paged_many(const pg_
                     }
                 }
                 __builtin_amdgcn_s_setprio(0);
+                float vsc[4];                    /* of the weights of each wavefront's keys: 2^(ev - Ev) */
+                if constexpr (F32) {
+                    int ev[4], any = Ev, top = Ev;
+#pragma unroll
+                    for (int g = 0; g < 4; g++) {
+                        const int x = __builtin_amdgcn_readfirstlane(scale_s[turn & 3][g]);
+                        any |= x;
+                        ev[g] = x >> 16;
+                        top = max(top, ev[g]);
+                    }
+                    if (any) {
+#pragma unroll
+                        for (int i = 0; i < 16; i++) st[0][i] = ldexpf(st[0][i], (int16_t)scale_s[turn & 3][i >> 2]);
+#pragma unroll
+                        for (int d = 0; d < ND; d++)
+#pragma unroll
+                            for (int i = 0; i < 16; i++) o[d][i] = ldexpf(o[d][i], Ev - top);
+                    }
+                    Ev = top;
+#pragma unroll
+                    for (int g = 0; g < 4; g++) vsc[g] = __int_as_float((127 + max(ev[g] - top, -127)) << 23);
+                }
                 const bool edge = jb < wfull || jb + KT - 1 > wfirst;
                 if (edge)
 #pragma unroll
@@ -420,7 +486,12 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_paged_many(const pg_
                         l += x;
                         l += y;
                         uint32_t wd[NQ];
-                        pg_pieces2<OT, NQ>(x, y, wd);
+                        if constexpr (F32) {
+                            const float f = vsc[2 * (k & 1) + (i >> 1)];
+                            pg_pieces2<OT, NQ>(x * f, y * f, wd);
+                        } else {
+                            pg_pieces2<OT, NQ>(x, y, wd);
+                        }
 #pragma unroll
                         for (int p = 0; p < NQ; p++) {
                             if (i == 0) pf[k & 1][p].x = wd[p];
@@ -503,6 +574,7 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_paged_many(const pg_
             if (more) {
                 if constexpr (F32) {
                     note(n + 1, buf ^ 1, turn + 1);
+                    scale(turn + 1);
                     store(buf ^ 1);
                 } else {
                     wait_vm_lgkm<0>();
@@ -518,6 +590,11 @@ __global__ __launch_bounds__(256, HD <= 128 ? 2 : 1) void k_paged_many(const pg_
             turn++;
         }
         l = pg_half_sum(l);
+        if (F32 && Ev != 0)
+#pragma unroll
+            for (int d = 0; d < ND; d++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) o[d][i] = ldexpf(o[d][i], Ev);
 
         /* ---- the rows: written, or left as a piece. A lane's elements 8 e + 4 h .. + 3 of its row */
         const pg_args *late = pg_late_args();

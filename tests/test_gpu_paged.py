@@ -223,6 +223,42 @@ def test_query_range(cpg, qs, ctype):
     b.close()
 
 
+@pytest.mark.parametrize("ks,vs", [(1e-30, 1e-30), (1e-5, 1e-4), (1e5, 1e6), (1e30, 1e30), (1.0, 1e-7), (1.0, 1e7)])
+@pytest.mark.parametrize("HD", [64, 128, 192])
+def test_cache_range(cpg, HD, ks, vs):
+    """f32 caches take any size of keys and values; the scores are of order one throughout"""
+    for seqs in ([(150, 1), (90, 60), (200, 33)], [(700, 40)]):
+        b = Batch(seqs, 2, HD, 16, F32).fill()
+        b.k *= np.float32(ks)
+        b.v *= np.float32(vs)
+        b.upload()
+        ws = Workspace(8, 2, HD)
+        q = queries(b, 8, F32, sigma=1 / ks)
+        out, lse = attend(b, ws, q, 8, F32)
+        assert ws.status() == 0
+        compare(b, q, 8, F32, out, lse)
+        ws.close()
+        b.close()
+
+
+@pytest.mark.parametrize("window", [0, 90])
+def test_cache_range_over_a_sequence(cpg, window):
+    """values that grow and fall over 2^40, keys over 2^8, from token to token, some of them zero"""
+    b = Batch([(640, 200), (640, 1)], 2, 64, 16, F32).fill()
+    for s in range(2):
+        for j in range(640):
+            w = b.where(s, j)
+            b.v[w] *= np.float32(2.0 ** (20 - abs(j - 320) / 8)) if j % 50 > 20 or j > 500 else np.float32(0)
+            b.k[w] *= np.float32(2.0 ** (j % 9 - 4))
+    b.upload()
+    ws = Workspace(4, 2, 64)
+    q = queries(b, 4, F32, sigma=0.1)
+    out, lse = attend(b, ws, q, 4, F32, window)
+    compare(b, q, 4, F32, out, lse, window)
+    ws.close()
+    b.close()
+
+
 @pytest.mark.parametrize("type_,ctype", COMBOS)
 @pytest.mark.parametrize("window", [0, 30])
 def test_what_a_row_does_not_see_does_not_reach_it(cpg, type_, ctype, window):
