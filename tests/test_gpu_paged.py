@@ -672,6 +672,60 @@ def test_graph_replays_as_the_batch_moves(cpg):
     b.close()
 
 
+def test_two_graphs_over_one_workspace(cpg):
+    """a graph of decode steps and one of prompts, with the same workspace, replayed in turn"""
+    H, KV, HD = 8, 2, 128
+    ws, L = Workspace(H, KV, HD), C.lib()
+    made = []
+    for seqs in ([(900, 1), (60, 1), (2500, 1)], [(700, 300), (64, 64), (1200, 90)]):
+        b = Batch(seqs, KV, HD, 16, BF16).fill().upload()
+        q = queries(b, H, BF16)
+        want, _ = attend(b, ws, q, H, BF16)
+        dq, do = C.to_device(to_type(q, BF16)), C.DeviceBuffer(b.T * H * HD * 2)
+        cache, batch = b.cache(), b.batch()
+
+        def enqueue():
+            C.check(L.cpg_paged_attn(ctypes.byref(cache), ctypes.byref(batch), BF16, H, dq.ptr, H * HD, 0.0, 0,
+                                     do.ptr, H * HD, None, ws.ptr), "attn")
+
+        C.check(L.cpg_capture_begin(), "capture")
+        enqueue()
+        graph = L.cpg_capture_end()
+        assert graph, C.last_error()
+        made.append((b, dq, do, graph, want))
+    for turn in range(4):
+        for b, dq, do, graph, want in made:
+            do.zero()
+        for b, dq, do, graph, want in made + made:   # no synchronisation between them
+            C.check(L.cpg_graph_launch(graph), "launch")
+        C.sync()
+        for b, dq, do, graph, want in made:
+            got = do.download(np.uint16, b.T * H * HD).reshape(want.shape)
+            assert np.array_equal(got, want), turn
+    assert ws.status() == 0
+    for b, dq, do, graph, want in made:
+        L.cpg_graph_destroy(graph)
+        for d in (dq, do, b):
+            d.close()
+    ws.close()
+
+
+@pytest.mark.parametrize("type_,ctype", [(F32, F32), (BF16, BF16)])
+def test_sequences_that_share_pages(cpg, type_, ctype):
+    """a prefix held once by three sequences, and a page that a sequence has twice"""
+    b = Batch([(200, 20), (180, 1), (170, 3), (96, 40)], 2, 64, 16, ctype).fill()
+    b.pages[1, :8] = b.pages[2, :8] = b.pages[0, :8]
+    b.pages[3, 3] = b.pages[3, 1]
+    b.upload()
+    ws = Workspace(8, 2, 64)
+    q = queries(b, 8, type_)
+    out, lse = attend(b, ws, q, 8, type_)
+    assert ws.status() == 0
+    compare(b, q, 8, type_, out, lse)
+    ws.close()
+    b.close()
+
+
 @pytest.mark.parametrize("ctype", [F32, BF16])
 def test_serving_steps_against_the_layer(cpg, ctype):
     """Two conversations served together through the paged cache (projection, append, attention, output
