@@ -18,8 +18,13 @@
  * 16-bit caches are copied into LDS by the memory pipe itself (global_load_lds_dwordx4); the
  * exchange of chunks is made by permuting the addresses a lane reads from. f32 caches pass
  * through registers, where each element becomes two f16 (hi and lo, 22 bits): products of K and Q,
- * V and P are then three (hi hi + hi lo + lo hi). f32 queries over 16-bit caches are two f16 or three
- * bf16 pieces (rows of queries scaled by a power of two into f16's range), and so are the weights.
+ * V and P are then three (hi hi + hi lo + lo hi). So that f16's exponents reach, the keys and the
+ * values that a wavefront stages (a quarter of the step's, eight tokens) go by powers of two where
+ * their largest element is not within 2^-3 .. 2^15: the scores take the keys' back, the weights and
+ * the accumulators the values' (3 % of the time; without it, values of 1e-4 were off by 3e-5 of
+ * the largest, and what passed 65504 became NaN). f32 queries over 16-bit caches are two f16 or
+ * three bf16 pieces (rows of queries scaled by a power of two into f16's range), and so are the
+ * weights.
  *
  * The running maximum that the weights refer to is renewed only where a score passes it by 2^8: until
  * then weights above one are as good (their sum and the accumulators are fp32), and most of the
@@ -27,6 +32,9 @@
  *
  * What bounds it: the matrix products and the softmax's vector work (exp2, maximum, sum, rounding:
  * about as many cycles as the products of 16-bit operands), the two workgroups of a CU in turn.
+ * Prompts of 1500 - 4500 tokens, bf16, 32 heads of 128 on 8: 240 us, 830 TFLOP/s (a large library
+ * product: 1136), matrix units busy 38 % of the cycles; 512 tokens over 3584, f32, 32 heads on 4: 120
+ * us, 270 TFLOP/s, 810 with the three products of each, matrix units busy 35 %.
  */
 #include "cpg_paged.h"
 

@@ -396,9 +396,10 @@ int cpg_paged_append(const cpg_paged_cache *C, const cpg_paged_batch *B, const c
    it, whatever they hold. Sums, softmax and accumulation are fp32; scores and weights are products
    of matrix instructions, of f32 over an f32 cache, of f16 or bf16 over a 16-bit one: f32
    activations in pieces that keep 22 or more bits of them, 16-bit activations with the weights
-   rounded to 16 bits. (k_paged_many takes an f32 cache as pairs of f16: keys and values beyond
-   65504 become infinite there.) The way the sums are split depends on the batch, and with it the
-   last bits; the same call gives the same bits. out may not overlap q. Asynchronous. */
+   rounded to 16 bits. (k_paged_many takes an f32 cache as pairs of f16, an element to 2^-22 of
+   itself or of the largest among eight neighbouring tokens. An infinite element makes what it
+   reaches infinite or NaN.) The way the sums are split depends on the batch, and with
+   it the last bits; the same call gives the same bits. out may not overlap q. Asynchronous. */
 int cpg_paged_attn(const cpg_paged_cache *C, const cpg_paged_batch *B, int type, int H,
                    const void *q, int64_t ldq, float scale, int window, void *out, int64_t ldo,
                    float *lse, cpg_paged_ws *ws);
